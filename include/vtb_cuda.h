@@ -45,6 +45,8 @@ extern "C" {
 #define VTB_CUDA_ERR_COMM (-10)
 
 #define VTB_CUDA_F32 0
+#define VTB_CUDA_F16 1   /* paged cache and its rows only */
+#define VTB_CUDA_BF16 30 /* paged cache and its rows only */
 #define VTB_CUDA_Q8_0 8
 #define VTB_CUDA_Q4_K 12
 #define VTB_CUDA_Q5_K 13
@@ -158,6 +160,95 @@ int vtb_cuda_gemm(int quant, const void *w, const float *acts, float *out, int64
 #define VTB_CUDA_NOALLOC_MAX_K 65536
 int vtb_cuda_gemv_q8_0_q8_0_noalloc(const void *w, const float *x, float *y, int64_t m, int64_t k,
                                     void *stream, int pdl);
+
+/* ------------------------------------------------------------------ */
+/* Paged key-value cache (device pointers)                              */
+/* ------------------------------------------------------------------ */
+
+/* One layer's cache cut into pages of `page_size` positions, so sequences
+ * take memory as they grow, share the pages of a common prefix, and give back
+ * pages that a sliding window has left.  The reference has one contiguous
+ * cache per session (src/runtime/kv_cache.zig:20-73).
+ *
+ * Position t of sequence s lies in page page_table[s * table_stride + t / page_size],
+ * slot t % page_size; value d of kv head h there is
+ *   k[page * page_stride + h * head_stride + slot * slot_stride + d]   (elements)
+ * and the same in v.  Any order of the three strides works; [page][head][slot]
+ * keeps a head's positions together, which reads fastest.  k, v and every
+ * stride in bytes are multiples of 16; page_size is a power of two up to 1024;
+ * head_dim is 64 or 128; type is F32, F16 or BF16.
+ *
+ * Page ids are read only where a position is written or visible, so entries of
+ * unused or evicted pages may hold anything (-1).  An id outside [0, n_pages)
+ * that is read, a length or position beyond the table, or a row list that does
+ * not fit sets the device error word (vtb_cuda_check_device_error); the calls
+ * stay in bounds, and what the affected rows hold is unspecified. */
+typedef struct VtbCudaPagedKv {
+  void *k, *v;
+  int32_t type, n_kv_heads, head_dim, page_size;
+  int64_t n_pages, page_stride, head_stride, slot_stride;
+  const int32_t *page_table; /* device [n_seqs][table_stride], the first pages_per_seq of a row used */
+  int64_t table_stride;
+  int32_t n_seqs, pages_per_seq;
+} VtbCudaPagedKv;
+
+/* New rows for the cache (f32 or the cache's type): value d of head h of row r
+ * is x[r * x_row_stride + h * x_head_stride + d].  With `rope` ([n_rope][head_dim]
+ * f32, (cos, sin) of pair i of position p at [p][2i], [p][2i + 1]) keys and
+ * queries are rotated by interleaved pairs (math.zig:88-104) at the row's
+ * position before they are rounded to the cache's type. */
+typedef struct VtbCudaPagedRows {
+  int32_t type, n_heads;
+  int64_t n_rows;
+  const void *k, *v, *q; /* q may be NULL */
+  int64_t k_row_stride, k_head_stride, v_row_stride, v_head_stride, q_row_stride, q_head_stride;
+  void *q_out;        /* [n_rows][n_heads][head_dim], the cache's type (NULL without q) */
+  const float *rope;  /* NULL: no rotation */
+  int64_t n_rope;
+  const int32_t *seq, *pos; /* device [n_rows]; a negative one skips the row */
+} VtbCudaPagedRows;
+
+/* Writes rows' keys and values at (seq, pos) and their queries to q_out.  Each
+ * (seq, pos) may be listed once; q_out may be q itself when types and strides
+ * agree. */
+int vtb_cuda_paged_append(const VtbCudaPagedKv *kv, const VtbCudaPagedRows *rows, void *stream);
+
+/* Attention over the pages.  q and out are of the cache's type; n_heads is a
+ * multiple of n_kv_heads (query head h reads kv head h / (n_heads / n_kv_heads)).
+ * lens[s] counts the cached positions of sequence s, the new ones included.  A
+ * query at position p sees t <= p, with window > 0 only t > p - window or
+ * t < sinks.  Softmax and sums are in f32.  A query that sees nothing gets zeros. */
+typedef struct VtbCudaPagedAttn {
+  const void *q;
+  void *out;
+  int64_t q_row_stride, q_head_stride, out_row_stride, out_head_stride; /* elements, whole 16 bytes */
+  int32_t n_heads, window, sinks;
+  float scale;
+  const int32_t *lens; /* device [n_seqs] */
+  void *workspace;     /* 16-byte aligned; calls that may overlap need one each */
+  size_t workspace_bytes;
+} VtbCudaPagedAttn;
+
+size_t vtb_cuda_paged_attn_workspace_bytes(int type, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim);
+
+/* Decode: row s of q is the one new token of sequence s, at position lens[s] - 1. */
+int vtb_cuda_paged_attn_decode(const VtbCudaPagedKv *kv, const VtbCudaPagedAttn *attn, void *stream);
+
+/* Prefill: rows [starts[s], starts[s + 1]) of q are the last new tokens of
+ * sequence s, at positions lens[s] - n ... lens[s] - 1 (starts: device
+ * [n_seqs + 1], within [0, n_rows]).  Their keys and values are in the cache
+ * already.  Rows that no sequence holds are left as they were. */
+int vtb_cuda_paged_attn_prefill(const VtbCudaPagedKv *kv, const VtbCudaPagedAttn *attn, const int32_t *starts,
+                                int64_t n_rows, void *stream);
+
+/* Copies page src[i] to page dst[i], K and V, in n_layers layers that lie
+ * layer_stride elements apart (a fork's private copies, a compaction's moves).
+ * No page may be a target twice, or a target and a source.  With page_table and
+ * page_map ([n_pages]), every entry e >= 0 of the kv's n_seqs x pages_per_seq
+ * table becomes page_map[e] in the same launch. */
+int vtb_cuda_paged_copy(const VtbCudaPagedKv *kv, int32_t n_layers, int64_t layer_stride, const int32_t *src,
+                        const int32_t *dst, int64_t n_moves, int32_t *page_table, const int32_t *page_map,
+                        void *stream);
 
 /* ------------------------------------------------------------------ */
 /* Context / buffers (mirrors the Metal bridge, bridge.h:25-46)         */

@@ -38,6 +38,11 @@ SIGNATURES = {
     "vtb_cuda_gemv_q8_0_q8_0_noalloc": (_int, [_vp, _vp, _vp, _i64, _i64, _vp, _int]),
     "vtb_cuda_gemm_workspace_bytes": (_sz, [_i64, _i64, _int]),
     "vtb_cuda_gemm": (_int, [_int, _vp, _vp, _vp, _i64, _i64, _i64, _int, _vp, _sz, _vp]),
+    "vtb_cuda_paged_append": (_int, [_vp, _vp, _vp]),
+    "vtb_cuda_paged_attn_workspace_bytes": (_sz, [_int, _i32, _i32, _i32]),
+    "vtb_cuda_paged_attn_decode": (_int, [_vp, _vp, _vp]),
+    "vtb_cuda_paged_attn_prefill": (_int, [_vp, _vp, _vp, _i64, _vp]),
+    "vtb_cuda_paged_copy": (_int, [_vp, _i32, _i64, _vp, _vp, _i64, _vp, _vp, _vp]),
     "vtb_cuda_capabilities": (_int, [_vp, _vp]),
     "vtb_cuda_init": (_vp, [_int]),
     "vtb_cuda_destroy": (None, [_vp]),
@@ -112,6 +117,28 @@ SIGNATURES = {
 class SamplerConfig(C.Structure):
     """VtbCudaSamplerConfig: the reference's VtbSamplerConfig (include/vantablack.h:46-51)."""
     _fields_ = [("temperature", C.c_float), ("top_k", C.c_size_t), ("top_p", C.c_float), ("seed", C.c_uint64)]
+
+
+class PagedKv(C.Structure):
+    """VtbCudaPagedKv."""
+    _fields_ = [("k", _vp), ("v", _vp), ("type", _i32), ("n_kv_heads", _i32), ("head_dim", _i32), ("page_size", _i32),
+                ("n_pages", _i64), ("page_stride", _i64), ("head_stride", _i64), ("slot_stride", _i64),
+                ("page_table", _vp), ("table_stride", _i64), ("n_seqs", _i32), ("pages_per_seq", _i32)]
+
+
+class PagedRows(C.Structure):
+    """VtbCudaPagedRows."""
+    _fields_ = [("type", _i32), ("n_heads", _i32), ("n_rows", _i64), ("k", _vp), ("v", _vp), ("q", _vp),
+                ("k_row_stride", _i64), ("k_head_stride", _i64), ("v_row_stride", _i64), ("v_head_stride", _i64),
+                ("q_row_stride", _i64), ("q_head_stride", _i64), ("q_out", _vp), ("rope", _vp), ("n_rope", _i64),
+                ("seq", _vp), ("pos", _vp)]
+
+
+class PagedAttn(C.Structure):
+    """VtbCudaPagedAttn."""
+    _fields_ = [("q", _vp), ("out", _vp), ("q_row_stride", _i64), ("q_head_stride", _i64), ("out_row_stride", _i64),
+                ("out_head_stride", _i64), ("n_heads", _i32), ("window", _i32), ("sinks", _i32), ("scale", C.c_float),
+                ("lens", _vp), ("workspace", _vp), ("workspace_bytes", _sz)]
 
 
 class VtbError(RuntimeError):

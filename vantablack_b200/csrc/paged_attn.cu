@@ -1,0 +1,559 @@
+// paged_attn.cu -- attention over the paged key-value cache: one new token
+// per sequence (decode), and a chunk of new tokens per sequence (prefill),
+// both with a sliding window and sinks (first positions that stay visible).
+//
+//   o = sum_t softmax_t(scale q . k_t) v_t over the visible t:
+//   t <= p, t < len, and (window == 0 or t > p - window or t < sinks)
+//
+// for a query at position p; a query that sees nothing gives 0.
+#include "paged.cuh"
+
+namespace vtb {
+
+struct AttnArgs {
+  PagedView kv;
+  const void* q;
+  void* out;
+  long long q_row, q_head, o_row, o_head;  // elements
+  const int32_t* lens;
+  const int32_t* starts;  // prefill: first row of each sequence, then the number of rows
+  int rows, n_kv, group, window, sinks;
+  float scale2;  // scale * log2(e): scores are kept in units of log2
+  float* part;   // partial results of splits
+};
+
+// A run of cached positions as one index range: `ns` sinks, then [w0, end).
+struct Span {
+  int ns, w0, n;
+  __device__ __forceinline__ int pos(int i) const { return i < ns ? i : i - ns + w0; }
+};
+// Positions that queries at [p0, p1] see (p0 <= p1; p1 < 0: none).
+__device__ __forceinline__ Span span_of(int p0, int p1, int window, int sinks) {
+  Span s{0, 0, 0};
+  if (p1 < 0) return s;
+  if (window && p0 >= window) s.w0 = p0 + 1 - window;
+  s.ns = min(sinks, s.w0);
+  s.n = s.ns + p1 + 1 - s.w0;
+  return s;
+}
+
+// ======================= decode =======================
+// HBM bound: K and V are read once.  The visible positions of every (sequence,
+// kv head) are cut into tiles of 64, all tiles put in one line, and the line
+// cut into equal parts, one per resident CTA: a ragged batch and a single long
+// sequence load the GPU the same way, with no host knowledge of the lengths
+// (a captured call stays right as they grow).  A part that covers a whole
+// (sequence, kv head) writes its output; the others leave (max, sum, o) behind
+// and decode_join_kernel adds them in line order, so results do not depend on
+// timing.  Each of the CTA's four warps streams its own 16 positions of a tile
+// through a private cp.async ring, with no barrier but at a part's end.
+constexpr int DT = 64, DWARPS = 4;
+
+template <typename T, int HD, int NT> struct DecodeCfg {
+  using S = Step<T, HD, NT>;
+  static constexpr int STAGE = 16 * (S::KROW + S::VROW);  // bytes: one warp's K and V rows
+  static constexpr int STAGES = 3;
+  static constexpr int RED = DWARPS * 8 * (HD + 4) * 4;
+  static constexpr int SMEM = DWARPS * STAGES * STAGE + RED + DWARPS * 8 * 2 * 4;
+  static constexpr int SLOT = NT * 8 * (HD + 2);  // floats of one partial result
+};
+
+struct Line {  // the line of all tiles, and this CTA's place in it
+  long long total;
+  int parts;
+};
+__device__ __forceinline__ int seq_tiles(const AttnArgs& a, int s) {
+  const int len = paged_len(a.kv, a.lens, s);
+  return (span_of(len - 1, len - 1, a.window, a.sinks).n + DT - 1) / DT;
+}
+__device__ __forceinline__ Line line_of(const AttnArgs& a, int units, int grid) {
+  long long n = 0;
+  for (int s = threadIdx.x & 31; s < a.kv.n_seqs; s += 32) n += seq_tiles(a, s);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  n *= units;
+  return Line{n, (int)(n < grid ? n : grid)};
+}
+// The sequence that holds place `w` of the line, and the tiles before it.
+__device__ __forceinline__ int line_seq(const AttnArgs& a, int units, long long w, long long& before) {
+  before = 0;
+  const int lane = threadIdx.x & 31;
+  for (int s0 = 0; s0 < a.kv.n_seqs; s0 += 32) {
+    long long n = s0 + lane < a.kv.n_seqs ? (long long)seq_tiles(a, s0 + lane) * units : 0, incl = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, before + incl > w);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      before += __shfl_sync(0xffffffffu, incl - n, l);
+      return s0 + l;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return -1;
+}
+
+struct LineCursor {  // one tile of the line
+  int s, u, t, nt;
+  Span sp;
+  __device__ __forceinline__ void enter(const AttnArgs& a) {
+    const int len = paged_len(a.kv, a.lens, s);
+    sp = span_of(len - 1, len - 1, a.window, a.sinks);
+    nt = (sp.n + DT - 1) / DT;
+  }
+  __device__ __forceinline__ void next(const AttnArgs& a, int units) {
+    if (++t < nt) return;
+    t = 0;
+    if (++u < units) return;
+    u = 0;
+    do ++s;
+    while (s < a.kv.n_seqs && (enter(a), nt == 0));
+  }
+};
+
+template <typename T, int HD, int NT>
+__global__ void __launch_bounds__(DWARPS * 32, Elem<T>::f32 ? 1 : 2)
+paged_decode_kernel(const __grid_constant__ AttnArgs a, int hgroups) {
+  using C = DecodeCfg<T, HD, NT>;
+  using S = Step<T, HD, NT>;
+  asm volatile("griddepcontrol.launch_dependents;");
+  extern __shared__ __align__(128) unsigned char smem[];
+  float* red = reinterpret_cast<float*>(smem + DWARPS * C::STAGES * C::STAGE);  // [warp][8][HD + 4]
+  float2* ml = reinterpret_cast<float2*>(red + DWARPS * 8 * (HD + 4));          // [warp][8]
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int units = a.n_kv * hgroups;
+  T* out = static_cast<T*>(a.out);
+  // sequences that see nothing
+  for (int s = blockIdx.x; s < a.kv.n_seqs; s += gridDim.x)
+    if (seq_tiles(a, s) == 0)
+      for (int i = threadIdx.x; i < a.n_kv * a.group * HD; i += DWARPS * 32)
+        out[s * a.o_row + (i / HD) * a.o_head + i % HD] = from_f<T>(0.f);
+  const Line line = line_of(a, units, gridDim.x);
+  if ((int)blockIdx.x >= line.parts) return;
+  const long long w0 = line.total * blockIdx.x / line.parts, w1 = line.total * (blockIdx.x + 1) / line.parts;
+  LineCursor cur;
+  long long before;
+  cur.s = line_seq(a, units, w0, before);
+  cur.enter(a);
+  cur.u = (int)((w0 - before) / cur.nt);
+  cur.t = (int)((w0 - before) % cur.nt);
+  LineCursor ld = cur;
+  const int n = (int)(w1 - w0);
+
+  const uint32_t ring = smem_u32(smem) + warp * C::STAGES * C::STAGE;
+  // The row this lane looks up for the next tile to load (rows lane & 15), and its page:
+  // the table is read one tile ahead of the copies that need it.
+  int row_pos = -1, row_page = 0;
+  auto look = [&]() {
+    const int i = ld.t * DT + warp * 16 + (lane & 15);
+    row_pos = -1;
+    if (ld.s < a.kv.n_seqs && i < ld.sp.n) {
+      row_pos = ld.sp.pos(i);
+      row_page = a.kv.table[ld.s * a.kv.table_stride + (row_pos >> a.kv.page_shift)];
+    }
+  };
+  auto load = [&](int stage) {
+    const long long off = row_pos < 0 ? -1 : page_row(a.kv, row_page, row_pos) + (ld.u / hgroups) * a.kv.head_stride;
+    const uint32_t kd = ring + stage * C::STAGE, vd = kd + 16 * S::KROW;
+    constexpr int RPI = 32 / S::PIECES > 0 ? 32 / S::PIECES : 1;  // rows per round of 32 lanes
+#pragma unroll
+    for (int r0 = 0; r0 < 16; r0 += RPI) {
+      const int r = r0 + lane / S::PIECES, pc = lane % S::PIECES;
+      const long long o = __shfl_sync(0xffffffffu, off, r);
+      const long long src = (o < 0 ? 0 : o) + pc * 16;
+      cpa16(kd + S::k_off(r, pc), a.kv.k + src, o >= 0);
+      cpa16(vd + S::v_off(r, pc), a.kv.v + src, o >= 0);
+    }
+  };
+  look();
+#pragma unroll
+  for (int i = 0; i < C::STAGES - 1; ++i) {
+    if (i < n) {
+      load(i);
+      ld.next(a, units);
+      if (i + 1 < n) look();
+    }
+    cpa_commit();
+  }
+
+  S st;
+  float m[NT][2], l[NT][2], o[NT][HD / 16][4];
+  bool fresh = true, first_part = true;
+  for (int i = 0; i < n; ++i) {
+    if (fresh) {
+      fresh = false;
+      const T* q = static_cast<const T*>(a.q) + cur.s * a.q_row;
+      const int h0 = (cur.u % hgroups) * NT * 8, kvh = cur.u / hgroups;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int h = h0 + 8 * nt + g;
+        st.load_q(nt, h < a.group ? q + (long long)(kvh * a.group + h) * a.q_head : nullptr, t);
+        m[nt][0] = m[nt][1] = -INFINITY;
+        l[nt][0] = l[nt][1] = 0.f;
+#pragma unroll
+        for (int j = 0; j < HD / 16; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
+      }
+    }
+    cpa_wait<C::STAGES - 2>();
+    __syncwarp();
+    if (i + C::STAGES - 1 < n) {
+      load((i + C::STAGES - 1) % C::STAGES);
+      ld.next(a, units);
+      if (i + C::STAGES < n) look();
+    }
+    cpa_commit();
+    const int base = cur.t * DT + warp * 16;
+    if (base < cur.sp.n) {
+      const uint32_t kb = ring + (i % C::STAGES) * C::STAGE;
+      float s[NT][4];
+      st.scores(kb, lane, s);
+      const bool in0 = base + g < cur.sp.n, in1 = base + g + 8 < cur.sp.n;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        s[nt][0] = in0 ? s[nt][0] * a.scale2 : -INFINITY;
+        s[nt][1] = in0 ? s[nt][1] * a.scale2 : -INFINITY;
+        s[nt][2] = in1 ? s[nt][2] * a.scale2 : -INFINITY;
+        s[nt][3] = in1 ? s[nt][3] * a.scale2 : -INFINITY;
+      }
+      softmax_step<NT, HD / 16>(s, m, l, o);
+      st.pv(kb + 16 * S::KROW, lane, s, o);
+    }
+    if (cur.t + 1 < cur.nt && i + 1 < n) {
+      ++cur.t;
+      continue;
+    }
+    // ---- end of this CTA's share of (sequence, unit): join the four warps ----
+    fresh = true;
+    const bool whole = cur.t + 1 == cur.nt && i >= cur.nt - 1;
+    const int h0 = (cur.u % hgroups) * NT * 8, kvh = cur.u / hgroups;
+    float* slot = a.part + (2ll * blockIdx.x + (first_part ? 0 : 1)) * C::SLOT;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], off);
+        if (g == 0) ml[warp * 8 + 2 * t + c] = make_float2(m[nt][c], l[nt][c]);
+      }
+      __syncthreads();
+      float f[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        float M = -INFINITY;
+        for (int w = 0; w < DWARPS; ++w) M = fmaxf(M, ml[w * 8 + 2 * t + c].x);
+        f[c] = exp2f(m[nt][c] - (M == -INFINITY ? 0.f : M));
+      }
+      float* mine = red + (warp * 8 + 2 * t) * (HD + 4);
+#pragma unroll
+      for (int j = 0; j < HD / 16; ++j)
+#pragma unroll
+        for (int hi = 0; hi < 2; ++hi) {
+          const int d = S::dim(j, hi, g);
+          mine[d] = o[nt][j][2 * hi] * f[0];
+          mine[HD + 4 + d] = o[nt][j][2 * hi + 1] * f[1];
+        }
+      __syncthreads();
+      const int heads = min(8, a.group - h0 - 8 * nt);
+      for (int x = threadIdx.x; x < heads * HD; x += DWARPS * 32) {
+        const int h = x / HD, d = x % HD;
+        float M = -INFINITY, L = 0.f, acc = 0.f;
+        for (int w = 0; w < DWARPS; ++w) M = fmaxf(M, ml[w * 8 + h].x);
+        const float b = M == -INFINITY ? 0.f : M;
+        for (int w = 0; w < DWARPS; ++w) {
+          const float2 v = ml[w * 8 + h];
+          L += v.y * exp2f(v.x - b);
+          acc += red[(w * 8 + h) * (HD + 4) + d];
+        }
+        if (whole) {
+          out[cur.s * a.o_row + (long long)(kvh * a.group + h0 + 8 * nt + h) * a.o_head + d] =
+              from_f<T>(L == 0.f ? 0.f : acc / L);
+        } else {
+          slot[NT * 16 + (8 * nt + h) * HD + d] = acc;
+          if (d == 0) {
+            slot[8 * nt + h] = M;
+            slot[NT * 8 + 8 * nt + h] = L;
+          }
+        }
+      }
+      __syncthreads();  // ml and red are free again
+    }
+    first_part = false;
+    cur.next(a, units);
+  }
+  cpa_wait<0>();
+}
+
+// Adds the parts of each (sequence, unit) that a boundary of the line cuts: CTA
+// b looks at boundary b + 1 and works only if it is the first one in its unit.
+template <typename T, int HD, int NT>
+__global__ void __launch_bounds__(256) paged_decode_join_kernel(const __grid_constant__ AttnArgs a, int hgroups, int grid) {
+  using C = DecodeCfg<T, HD, NT>;
+  const int units = a.n_kv * hgroups;
+  const Line line = line_of(a, units, grid);
+  const int c = blockIdx.x + 1;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (c >= line.parts) return;
+  const long long w = line.total * c / line.parts, prev = line.total * (c - 1) / line.parts;
+  long long before;
+  const int s = line_seq(a, units, w, before);
+  const int nt = seq_tiles(a, s);
+  const int u = (int)((w - before) / nt);
+  const long long u0 = before + (long long)u * nt, u1 = u0 + nt;
+  if (w == u0 || prev > u0) return;  // no cut here, or not the unit's first
+  int last = c;
+  while (last + 1 < line.parts && line.total * (last + 1) / line.parts < u1) ++last;
+  const float* p0 = a.part + (2ll * (c - 1) + (prev == u0 ? 0 : 1)) * C::SLOT;
+  const int h0 = (u % hgroups) * NT * 8, kvh = u / hgroups, heads = min(8 * NT, a.group - h0);
+  T* out = static_cast<T*>(a.out) + s * a.o_row + (long long)(kvh * a.group + h0) * a.o_head;
+  for (int x = threadIdx.x; x < heads * HD; x += blockDim.x) {
+    const int h = x / HD, d = x % HD;
+    float M = p0[h];
+    for (int i = c; i <= last; ++i) M = fmaxf(M, a.part[2ll * i * C::SLOT + h]);
+    const float b = M == -INFINITY ? 0.f : M;
+    float e = exp2f(p0[h] - b), L = p0[NT * 8 + h] * e, acc = p0[NT * 16 + h * HD + d] * e;
+#pragma unroll 4
+    for (int i = c; i <= last; ++i) {
+      const float* p = a.part + 2ll * i * C::SLOT;
+      e = exp2f(p[h] - b);
+      L += p[NT * 8 + h] * e;
+      acc += p[NT * 16 + h * HD + d] * e;
+    }
+    out[h * a.o_head + d] = from_f<T>(L == 0.f ? 0.f : acc / L);
+  }
+}
+
+// ======================= prefill =======================
+// The query rows of one kv head are the pairs (token, head of the group) in
+// token order, flattened, so any group size fills the 128 rows of a CTA; the
+// CTA walks the positions that its rows see in tiles of 64 staged through two
+// cp.async stages.  Warp w owns rows 16 w .. 16 w + 15.
+constexpr int PQ = 128, PT = 64, PWARPS = 8;
+
+template <typename T, int HD> struct PrefillCfg {
+  using S = Step<T, HD, 2>;
+  static constexpr int STAGE = PT * (S::KROW + S::VROW);
+  static constexpr int OUT = PWARPS * 16 * (HD + 4) * 4;
+  static constexpr int SMEM = 2 * STAGE > OUT ? 2 * STAGE : OUT;
+};
+
+// Rows [r0, r0 + n) of sequence s; tile `idx` of the line of all sequences' row
+// tiles gives (s, first flattened row).  Bad starts set the error word.
+struct RowTile {
+  int s, r0, n, f0, ctx;
+};
+__device__ __forceinline__ int chunk_rows(const AttnArgs& a, int s, int& r0) {
+  r0 = a.starts[s];
+  const int r1 = a.starts[s + 1];
+  if (r0 < 0 || r1 < r0 || r1 > a.rows) {
+    flag_error(DEV_ERR_BAD_ARG);
+    return 0;
+  }
+  return r1 - r0;
+}
+__device__ __forceinline__ bool row_tile(const AttnArgs& a, int idx, int tile, RowTile& rt) {
+  const int lane = threadIdx.x & 31;
+  long long before = 0;
+  for (int s0 = 0; s0 < a.kv.n_seqs; s0 += 32) {
+    int r0 = 0, n = 0;
+    if (s0 + lane < a.kv.n_seqs) n = chunk_rows(a, s0 + lane, r0);
+    const long long tiles = ((long long)n * a.group + tile - 1) / tile;
+    long long incl = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long x = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += x;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, before + incl > idx);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      rt.s = s0 + l;
+      rt.r0 = __shfl_sync(0xffffffffu, r0, l);
+      rt.n = __shfl_sync(0xffffffffu, n, l);
+      rt.f0 = (int)(idx - before - __shfl_sync(0xffffffffu, incl - tiles, l)) * tile;
+      rt.ctx = paged_len(a.kv, a.lens, rt.s) - rt.n;
+      return true;
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return false;
+}
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(PWARPS * 32, 1) paged_prefill_kernel(const __grid_constant__ AttnArgs a) {
+  using C = PrefillCfg<T, HD>;
+  using S = Step<T, HD, 2>;
+  extern __shared__ __align__(128) unsigned char smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  RowTile rt;
+  if (!row_tile(a, gridDim.x - 1 - blockIdx.x, PQ, rt)) return;
+  const int kvh = blockIdx.y, nflat = rt.n * a.group;
+  const int last = min(rt.f0 + PQ, nflat) - 1;
+  const Span sp = span_of(max(0, rt.ctx + rt.f0 / a.group), rt.ctx + last / a.group, a.window, a.sinks);
+  const int tiles = (sp.n + PT - 1) / PT;
+
+  const uint32_t sbase = smem_u32(smem);
+  auto load = [&](int tile) {
+    const uint32_t kd = sbase + (tile & 1) * C::STAGE, vd = kd + PT * S::KROW;
+    for (int x = threadIdx.x; x < PT * S::PIECES; x += PWARPS * 32) {
+      const int r = x / S::PIECES, pc = x % S::PIECES, i = tile * PT + r;
+      const bool live = i < sp.n;
+      long long src = pc * 16;
+      if (live) {
+        const int pos = sp.pos(i);
+        src += page_row(a.kv, a.kv.table[rt.s * a.kv.table_stride + (pos >> a.kv.page_shift)], pos) + kvh * a.kv.head_stride;
+      }
+      cpa16(kd + S::k_off(r, pc), a.kv.k + src, live);
+      cpa16(vd + S::v_off(r, pc), a.kv.v + src, live);
+    }
+  };
+  if (tiles > 0) load(0);
+  cpa_commit();
+
+  S st;
+  float m[2][2], l[2][2], o[2][HD / 16][4];
+  int qp[2][2];  // position of vectors 8 nt + 2t + c
+#pragma unroll
+  for (int nt = 0; nt < 2; ++nt) {
+    const int f = rt.f0 + warp * 16 + nt * 8;
+    const T* q = nullptr;
+    if (f + g < nflat)
+      q = static_cast<const T*>(a.q) + (rt.r0 + (f + g) / a.group) * a.q_row +
+          (long long)(kvh * a.group + (f + g) % a.group) * a.q_head;
+    st.load_q(nt, q, t);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const int fv = f + 2 * t + c;
+      qp[nt][c] = fv < nflat ? rt.ctx + fv / a.group : -1;
+      m[nt][c] = -INFINITY;
+      l[nt][c] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < HD / 16; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
+  }
+  for (int tile = 0; tile < tiles; ++tile) {
+    if (tile + 1 < tiles) load(tile + 1);
+    cpa_commit();
+    cpa_wait<1>();
+    __syncthreads();
+    const uint32_t kb = sbase + (tile & 1) * C::STAGE, vb = kb + PT * S::KROW;
+#pragma unroll 1
+    for (int r = 0; r < PT && tile * PT + r < sp.n; r += 16) {
+      float s[2][4];
+      st.scores(kb + S::k_off(r, 0), lane, s);
+#pragma unroll
+      for (int hi = 0; hi < 2; ++hi) {
+        const int i = tile * PT + r + g + 8 * hi, pos = i < sp.n ? sp.pos(i) : 0x7fffffff;
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const bool see = pos <= qp[nt][c] && (!a.window || pos > qp[nt][c] - a.window || pos < a.sinks);
+            s[nt][2 * hi + c] = see ? s[nt][2 * hi + c] * a.scale2 : -INFINITY;
+          }
+      }
+      softmax_step<2, HD / 16>(s, m, l, o);
+      st.pv(vb + S::v_off(r, 0), lane, s, o);
+    }
+    __syncthreads();
+  }
+  // ---- output through shared memory, whole rows ----
+  cpa_wait<0>();
+  __syncthreads();
+  float* mine = reinterpret_cast<float*>(smem) + warp * 16 * (HD + 4);
+#pragma unroll
+  for (int nt = 0; nt < 2; ++nt)
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int off = 4; off < 32; off <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], off);
+      const float inv = l[nt][c] == 0.f ? 0.f : 1.f / l[nt][c];
+#pragma unroll
+      for (int j = 0; j < HD / 16; ++j)
+#pragma unroll
+        for (int hi = 0; hi < 2; ++hi)
+          mine[(8 * nt + 2 * t + c) * (HD + 4) + S::dim(j, hi, g)] = o[nt][j][2 * hi + c] * inv;
+    }
+  __syncwarp();
+  T* out = static_cast<T*>(a.out);
+  for (int r = 0; r < 16; ++r) {
+    const int f = rt.f0 + warp * 16 + r;
+    if (f >= nflat) break;
+    T* row = out + (rt.r0 + f / a.group) * a.o_row + (long long)(kvh * a.group + f % a.group) * a.o_head;
+    for (int d = lane; d < HD; d += 32) row[d] = from_f<T>(mine[r * (HD + 4) + d]);
+  }
+}
+
+// ======================= launches =======================
+template <typename T, int HD, int NT>
+static cudaError_t launch_decode_t(const AttnArgs& a, int hgroups, int grid, cudaStream_t st) {
+  using C = DecodeCfg<T, HD, NT>;
+  const int dev = current_device();
+  cudaError_t e = ensure_smem_attr<paged_decode_kernel<T, HD, NT>>(dev, C::SMEM);
+  if (e) return e;
+  // no more CTAs than tiles there can be
+  const long long cap = (long long)a.kv.pages_per_seq << a.kv.page_shift;
+  const long long vis = a.window && a.window + (long long)a.sinks < cap ? a.window + (long long)a.sinks : cap;
+  const long long most = a.kv.n_seqs * (long long)a.n_kv * hgroups * ((vis + DT - 1) / DT);
+  if (most < grid) grid = (int)(most > 0 ? most : 1);
+  paged_decode_kernel<T, HD, NT><<<grid, DWARPS * 32, C::SMEM, st>>>(a, hgroups);
+  if ((e = cudaGetLastError())) return e;
+  if (vis <= DT || grid == 1) return cudaSuccess;  // one tile per unit: nothing is cut
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid - 1);
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_decode_join_kernel<T, HD, NT>, a, hgroups, grid);
+}
+
+// Resident CTAs that share a decode call's line, and the workspace they need.
+static int decode_grid(int type) { return sm_count(current_device()) * (type == F32 ? 1 : 2); }
+size_t paged_decode_workspace(int type, int group, int head_dim) {
+  const int nt = group > 8 ? 2 : 1;
+  return (size_t)2 * decode_grid(type) * nt * 8 * (head_dim + 2) * sizeof(float);
+}
+
+cudaError_t launch_paged_decode(int type, int head_dim, const AttnArgs& a, cudaStream_t st) {
+  const int nt = a.group > 8 ? 2 : 1, hgroups = (a.group + 8 * nt - 1) / (8 * nt), grid = decode_grid(type);
+#define VTB_DEC(TY, HD)                                                             \
+  return nt == 1 ? launch_decode_t<TY, HD, 1>(a, hgroups, grid, st) : launch_decode_t<TY, HD, 2>(a, hgroups, grid, st)
+  if (type == F32) {
+    if (head_dim == 64) VTB_DEC(float, 64);
+    VTB_DEC(float, 128);
+  }
+  if (type == T_F16) {
+    if (head_dim == 64) VTB_DEC(__half, 64);
+    VTB_DEC(__half, 128);
+  }
+  if (head_dim == 64) VTB_DEC(__nv_bfloat16, 64);
+  VTB_DEC(__nv_bfloat16, 128);
+#undef VTB_DEC
+}
+
+template <typename T, int HD>
+static cudaError_t launch_prefill_t(const AttnArgs& a, cudaStream_t st) {
+  using C = PrefillCfg<T, HD>;
+  cudaError_t e = ensure_smem_attr<paged_prefill_kernel<T, HD>>(current_device(), C::SMEM);
+  if (e) return e;
+  // row tiles: at most one ragged tile per sequence more than full ones
+  const long long tiles = (long long)a.rows * a.group / PQ + a.kv.n_seqs;
+  paged_prefill_kernel<T, HD><<<dim3((unsigned)tiles, a.n_kv), PWARPS * 32, C::SMEM, st>>>(a);
+  return cudaGetLastError();
+}
+
+cudaError_t launch_paged_prefill(int type, int head_dim, const AttnArgs& a, cudaStream_t st) {
+#define VTB_PRE(TY) return head_dim == 64 ? launch_prefill_t<TY, 64>(a, st) : launch_prefill_t<TY, 128>(a, st)
+  if (type == F32) VTB_PRE(float);
+  if (type == T_F16) VTB_PRE(__half);
+  VTB_PRE(__nv_bfloat16);
+#undef VTB_PRE
+}
+
+}  // namespace vtb

@@ -24,6 +24,7 @@ from __future__ import annotations
 import numpy as np
 
 F32, Q8_0, Q4_K, Q5_K, Q6_K, TQ2_0 = 0, 8, 12, 13, 14, 32
+F16, BF16 = 1, 30  # cache and row types of the paged key-value cache
 
 BLOCK_BYTES = {Q8_0: 34, Q4_K: 144, Q5_K: 176, Q6_K: 210, TQ2_0: 66}
 BLOCK_ELEMS = {Q8_0: 32, Q4_K: 256, Q5_K: 256, Q6_K: 256, TQ2_0: 256}
