@@ -137,3 +137,12 @@ def test_python_front_end_refuses_host_tensors(lib):
         ops.paged_attention_decode(torch.zeros(2, 8, 64), k, k, t, torch.zeros(2, dtype=torch.int32))
     with pytest.raises(ValueError):
         ops.paged_copy(k, k, t[0], t[1])
+
+
+def test_packed_descriptors_have_the_c_layout(lib):
+    from vantablack_b200 import ops
+    for packed, c in ((ops._KV, _lib.PagedKv), (ops._ROWS, _lib.PagedRows), (ops._ATTN, _lib.PagedAttn)):
+        assert packed.size == C.sizeof(c)
+        vals = [0.5 if t is C.c_float else i + 1 for i, (_, t) in enumerate(c._fields_)]
+        got = c.from_buffer_copy(packed.pack(*vals))
+        assert [getattr(got, n) for n, _ in c._fields_] == vals

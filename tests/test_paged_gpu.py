@@ -13,7 +13,7 @@ pytestmark = pytest.mark.gpu
 
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
 DTYPES = [F32, F16, BF16]
-P_ROUNDED = {"decode": False, "prefill": False}
+P_ROUNDED = {"decode": False, "prefill": True}  # 16-bit prefill: P is one value of the type
 
 
 def check_rows(got, cache, s, q, pos, scale, window, sinks, what):
@@ -222,7 +222,24 @@ def test_prefill_strides(dtype, layout):
 
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_prefill_large_scores(dtype):
-    run_prefill(P.Cache([400], 1, 64, 16, dtype, 26), [390], 4, 64, scale=2.0)
+    cache = P.Cache([400], 1, 64, 16, dtype, 26)
+    for scale in (2.0, -0.3):
+        run_prefill(cache, [390], 4, 64, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_zero_scale_is_the_mean(dtype):
+    cache = P.Cache([40, 200], 2, 64, 16, dtype, 30)
+    run_prefill(cache, [40, 33], 8, 64, scale=1e-30)
+    run_decode(cache, 8, 64, scale=1e-30)
+    q = torch.randn(2, 8, 64, device="cuda").to(dtype)
+    i32 = lambda *n: torch.tensor(n, dtype=torch.int32, device="cuda")  # noqa: E731
+    got = (ops.paged_attention_decode(q, cache.k, cache.v, cache.table, cache.d_lens, scale=0.0),
+           ops.paged_attention_prefill(q, cache.k, cache.v, cache.table, cache.d_lens, i32(0, 1, 2), scale=0.0))
+    for s in range(2):
+        mean = cache.v_rows[s].double().mean(0).repeat_interleave(4, 0)
+        for g in got:
+            assert torch.allclose(g[s].double().cpu(), mean, rtol=2 * P.EPS[dtype], atol=2 * P.EPS[dtype])
 
 
 def test_prefill_rows_before_the_first_position_give_zeros():

@@ -169,16 +169,27 @@ template <typename T, int HD, int NT> struct Step<T, HD, NT, false> {
       for (int nt = 0; nt < NT; ++nt) mma16<T>(s[nt], a, q[nt][2 * j], q[nt][2 * j + 1]);
     }
   }
-  __device__ __forceinline__ void pv(uint32_t vbase, int lane, const float (&p)[NT][4], float (&o)[NT][HD / 16][4]) const {
+  // o = o * f + V^T P^T (f: the factor of each of the lane's vectors; all 1 unless `moved`)
+  __device__ __forceinline__ void pv(uint32_t vbase, int lane, const float (&p)[NT][4], const float (&f)[NT][2], bool moved,
+                                     float (&o)[NT][HD / 16][4]) const {
+    if (moved) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < HD / 16; ++j) {
+          o[nt][j][0] *= f[nt][0]; o[nt][j][2] *= f[nt][0];
+          o[nt][j][1] *= f[nt][1]; o[nt][j][3] *= f[nt][1];
+        }
+    }
     uint32_t bh[NT][2], bl[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const uint32_t hi = pack2<T>(p[nt][2 * h], p[nt][2 * h + 1]);
-        const float2 f = unpack2<T>(hi);
+        const float2 r = unpack2<T>(hi);
         bh[nt][h] = movm(hi);
-        bl[nt][h] = movm(pack2<T>(p[nt][2 * h] - f.x, p[nt][2 * h + 1] - f.y));
+        bl[nt][h] = movm(pack2<T>(p[nt][2 * h] - r.x, p[nt][2 * h + 1] - r.y));
       }
     const int r = (lane & 7) + ((lane >> 4) << 3), pc = (lane >> 3) & 1;
 #pragma unroll
@@ -216,17 +227,18 @@ template <int HD, int NT> struct Step<float, HD, NT, true> {
       q[nt][4 * jj] = v.x; q[nt][4 * jj + 1] = v.y; q[nt][4 * jj + 2] = v.z; q[nt][4 * jj + 3] = v.w;
     }
   }
-  static __device__ __forceinline__ void mma3(float* c, const uint32_t* ah, const uint32_t* al, float b0, float b1) {
-    uint32_t h0, l0, h1, l1;
-    split_tf32(b0, h0, l0);
-    split_tf32(b1, h1, l1);
-    mma_tf32(c, al, h0, h1);
-    mma_tf32(c, ah, l0, l1);
-    mma_tf32(c, ah, h0, h1);
-  }
+  // The tensor cores add their products to the accumulator with truncation, so
+  // a long chain drifts by half a last place per step, all in one direction.
+  // Chains are therefore short: the small cross terms have accumulators of
+  // their own, the leading ones two, and o is updated by an ordinary f32 add.
   __device__ __forceinline__ void scores(uint32_t kbase, int lane, float (&s)[NT][4]) const {
+    float big[2][NT][4], small[2][NT][4];
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.f;
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) big[i][nt][c] = small[i][nt][c] = 0.f;
     const int g = lane >> 2, t = lane & 3;
 #pragma unroll
     for (int jj = 0; jj < HD / 16; ++jj) {
@@ -240,26 +252,45 @@ template <int HD, int NT> struct Step<float, HD, NT, true> {
         split_tf32(va[2 * cc + 1], ah[2], al[2]);
         split_tf32(vb[2 * cc + 1], ah[3], al[3]);
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma3(s[nt], ah, al, q[nt][4 * jj + 2 * cc], q[nt][4 * jj + 2 * cc + 1]);
+        for (int nt = 0; nt < NT; ++nt) {
+          uint32_t h0, l0, h1, l1;
+          split_tf32(q[nt][4 * jj + 2 * cc], h0, l0);
+          split_tf32(q[nt][4 * jj + 2 * cc + 1], h1, l1);
+          mma_tf32(small[0][nt], al, h0, h1);
+          mma_tf32(small[1][nt], ah, l0, l1);
+          mma_tf32(big[cc][nt], ah, h0, h1);
+        }
       }
     }
-  }
-  __device__ __forceinline__ void pv(uint32_t vbase, int lane, const float (&p)[NT][4], float (&o)[NT][HD / 16][4]) const {
-    const int g = lane >> 2, t = lane & 3;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      // P^T of positions 8h + 2t, 8h + 2t + 1 for vector g: the 32-bit tile is
-      // transposed as two tiles of 16-bit halves
-      float b0[NT], b1[NT];
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[nt][c] = (big[0][nt][c] + big[1][nt][c]) + (small[0][nt][c] + small[1][nt][c]);
+  }
+  __device__ __forceinline__ void pv(uint32_t vbase, int lane, const float (&p)[NT][4], const float (&f)[NT][2], bool,
+                                     float (&o)[NT][HD / 16][4]) const {
+    const int g = lane >> 2, t = lane & 3;
+    // P^T of positions 8h + 2t, 8h + 2t + 1 for vector g: the 32-bit tile is
+    // transposed as two tiles of 16-bit halves
+    uint32_t bh[2][NT][2], bl[2][NT][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const uint32_t x = __float_as_uint(p[nt][2 * h]), y = __float_as_uint(p[nt][2 * h + 1]);
         const uint32_t lo = movm(__byte_perm(x, y, 0x5410)), hi = movm(__byte_perm(x, y, 0x7632));
-        b0[nt] = __uint_as_float(__byte_perm(lo, hi, 0x5410));
-        b1[nt] = __uint_as_float(__byte_perm(lo, hi, 0x7632));
+        split_tf32(__uint_as_float(__byte_perm(lo, hi, 0x5410)), bh[h][nt][0], bl[h][nt][0]);
+        split_tf32(__uint_as_float(__byte_perm(lo, hi, 0x7632)), bh[h][nt][1], bl[h][nt][1]);
       }
 #pragma unroll
-      for (int jj = 0; jj < HD / 32; ++jj) {
+    for (int jj = 0; jj < HD / 32; ++jj) {
+      float c[2][NT][4];
+#pragma unroll
+      for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) c[cc][nt][0] = c[cc][nt][1] = c[cc][nt][2] = c[cc][nt][3] = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
         const float4 f0 = lds_f4(vbase + v_off(8 * h + 2 * t, g + 8 * jj));
         const float4 f1 = lds_f4(vbase + v_off(8 * h + 2 * t + 1, g + 8 * jj));
         const float va[4] = {f0.x, f0.y, f0.z, f0.w}, vb[4] = {f1.x, f1.y, f1.z, f1.w};
@@ -271,9 +302,19 @@ template <int HD, int NT> struct Step<float, HD, NT, true> {
           split_tf32(vb[2 * cc], ah[2], al[2]);
           split_tf32(vb[2 * cc + 1], ah[3], al[3]);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma3(o[nt][2 * jj + cc], ah, al, b0[nt], b1[nt]);
+          for (int nt = 0; nt < NT; ++nt) {
+            mma_tf32(c[cc][nt], al, bh[h][nt][0], bh[h][nt][1]);
+            mma_tf32(c[cc][nt], ah, bl[h][nt][0], bl[h][nt][1]);
+            mma_tf32(c[cc][nt], ah, bh[h][nt][0], bh[h][nt][1]);
+          }
         }
       }
+#pragma unroll
+      for (int cc = 0; cc < 2; ++cc)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[nt][2 * jj + cc][i] = fmaf(o[nt][2 * jj + cc][i], f[nt][i & 1], c[cc][nt][i]);
     }
   }
   static __device__ __forceinline__ int dim(int j, int hi, int g) { return 4 * (g + 8 * (j >> 1)) + 2 * (j & 1) + hi; }
@@ -281,10 +322,10 @@ template <int HD, int NT> struct Step<float, HD, NT, true> {
 
 // Online softmax of the warp's 16 scores per vector (in units of log2): m is
 // the running maximum, l this lane's share of the running sum.  A row whose
-// maximum is still -inf keeps p = 0.  On return s holds p; o has been rescaled.
-template <int NT, int NJ>
-__device__ __forceinline__ void softmax_step(float (&s)[NT][4], float (&m)[NT][2], float (&l)[NT][2], float (&o)[NT][NJ][4]) {
-  float a[NT][2];
+// maximum is still -inf keeps p = 0.  On return s holds p, f the factors that
+// o needs (all 1 unless the result is true, the same for the whole warp).
+template <int NT>
+__device__ __forceinline__ bool softmax_step(float (&s)[NT][4], float (&m)[NT][2], float (&l)[NT][2], float (&f)[NT][2]) {
   bool moved = false;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
@@ -294,22 +335,14 @@ __device__ __forceinline__ void softmax_step(float (&s)[NT][4], float (&m)[NT][2
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
       const float mn = fmaxf(m[nt][c], x), base = mn == -INFINITY ? 0.f : mn;
-      a[nt][c] = exp2f(m[nt][c] - base);
+      f[nt][c] = exp2f(m[nt][c] - base);
       moved |= mn != m[nt][c];
       m[nt][c] = mn;
       s[nt][c] = exp2f(s[nt][c] - base);
       s[nt][c + 2] = exp2f(s[nt][c + 2] - base);
-      l[nt][c] = l[nt][c] * a[nt][c] + (s[nt][c] + s[nt][c + 2]);
+      l[nt][c] = l[nt][c] * f[nt][c] + (s[nt][c] + s[nt][c + 2]);
     }
-  if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        o[nt][j][0] *= a[nt][0]; o[nt][j][2] *= a[nt][0];
-        o[nt][j][1] *= a[nt][1]; o[nt][j][3] *= a[nt][1];
-      }
-  }
+  return __any_sync(0xffffffffu, moved);
 }
 
 }  // namespace vtb

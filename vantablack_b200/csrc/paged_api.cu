@@ -39,6 +39,13 @@ static int paged_rows_ok(const void* p, int64_t row, int64_t head, int es, int64
   return VTB_CUDA_OK;
 }
 
+// One workspace serves both attention calls.
+static size_t paged_workspace(int type, int group, int head_dim) {
+  const size_t d = paged_decode_workspace(type, group, head_dim);
+  const size_t p = type == F32 ? 0 : paged_prefill_tc_workspace(head_dim);
+  return d > p ? d : p;
+}
+
 static int paged_attn_args(const VtbCudaPagedKv* kv, const VtbCudaPagedAttn* p, AttnArgs* a) {
   if (!p) return set_err(VTB_CUDA_ERR_INVALID_ARG, "null attention arguments");
   int rc = paged_view(kv, true, &a->kv);
@@ -65,7 +72,10 @@ static int paged_attn_args(const VtbCudaPagedKv* kv, const VtbCudaPagedAttn* p, 
   a->group = p->n_heads / kv->n_kv_heads;
   a->window = p->window;
   a->sinks = p->sinks;
+  a->negate = false;
   a->scale2 = (float)((double)p->scale * 1.4426950408889634);
+  if (!p->workspace || !aligned16(p->workspace) || p->workspace_bytes < paged_workspace(kv->type, a->group, kv->head_dim))
+    return set_err(VTB_CUDA_ERR_INVALID_ARG, "workspace is missing, misaligned or too small");
   a->part = static_cast<float*>(p->workspace);
   return VTB_CUDA_OK;
 }
@@ -74,7 +84,7 @@ extern "C" {
 
 size_t vtb_cuda_paged_attn_workspace_bytes(int type, int32_t n_heads, int32_t n_kv_heads, int32_t head_dim) {
   if (!paged_elem_bytes(type) || n_kv_heads < 1 || n_heads < 1 || n_heads % n_kv_heads) return 0;
-  return paged_decode_workspace(type, n_heads / n_kv_heads, head_dim);
+  return paged_workspace(type, n_heads / n_kv_heads, head_dim);
 }
 
 int vtb_cuda_paged_attn_decode(const VtbCudaPagedKv* kv, const VtbCudaPagedAttn* p, void* stream) {
@@ -82,9 +92,6 @@ int vtb_cuda_paged_attn_decode(const VtbCudaPagedKv* kv, const VtbCudaPagedAttn*
   AttnArgs a;
   int rc = paged_attn_args(kv, p, &a);
   if (rc) return rc;
-  if (!p->workspace || !aligned16(p->workspace) ||
-      p->workspace_bytes < paged_decode_workspace(kv->type, a.group, kv->head_dim))
-    return set_err(VTB_CUDA_ERR_INVALID_ARG, "workspace is missing, misaligned or too small");
   return cuda_status(launch_paged_decode(kv->type, kv->head_dim, a, (cudaStream_t)stream));
 }
 
@@ -99,7 +106,9 @@ int vtb_cuda_paged_attn_prefill(const VtbCudaPagedKv* kv, const VtbCudaPagedAttn
   if (n_rows == 0) return VTB_CUDA_OK;
   a.starts = starts;
   a.rows = (int)n_rows;
-  return cuda_status(launch_paged_prefill(kv->type, kv->head_dim, a, (cudaStream_t)stream));
+  cudaStream_t st = (cudaStream_t)stream;
+  return cuda_status(kv->type == F32 ? launch_paged_prefill_f32(kv->head_dim, a, st)
+                                     : launch_paged_prefill_tc(kv->type, kv->head_dim, a, st));
 }
 
 int vtb_cuda_paged_append(const VtbCudaPagedKv* kv, const VtbCudaPagedRows* r, void* stream) {

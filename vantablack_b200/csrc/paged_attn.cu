@@ -19,6 +19,7 @@ struct AttnArgs {
   const int32_t* starts;  // prefill: first row of each sequence, then the number of rows
   int rows, n_kv, group, window, sinks;
   float scale2;  // scale * log2(e): scores are kept in units of log2
+  bool negate;   // tensor-core prefill: the scale is negative (scale2 holds its size)
   float* part;   // partial results of splits
 };
 
@@ -218,8 +219,9 @@ paged_decode_kernel(const __grid_constant__ AttnArgs a, int hgroups) {
         s[nt][2] = in1 ? s[nt][2] * a.scale2 : -INFINITY;
         s[nt][3] = in1 ? s[nt][3] * a.scale2 : -INFINITY;
       }
-      softmax_step<NT, HD / 16>(s, m, l, o);
-      st.pv(kb + 16 * S::KROW, lane, s, o);
+      float f[NT][2];
+      const bool moved = softmax_step<NT>(s, m, l, f);
+      st.pv(kb + 16 * S::KROW, lane, s, f, moved, o);
     }
     if (cur.t + 1 < cur.nt && i + 1 < n) {
       ++cur.t;
@@ -454,8 +456,9 @@ __global__ void __launch_bounds__(PWARPS * 32, 1) paged_prefill_kernel(const __g
             s[nt][2 * hi + c] = see ? s[nt][2 * hi + c] * a.scale2 : -INFINITY;
           }
       }
-      softmax_step<2, HD / 16>(s, m, l, o);
-      st.pv(vb + S::v_off(r, 0), lane, s, o);
+      float f[2][2];
+      const bool moved = softmax_step<2>(s, m, l, f);
+      st.pv(vb + S::v_off(r, 0), lane, s, f, moved, o);
     }
     __syncthreads();
   }
@@ -548,12 +551,8 @@ static cudaError_t launch_prefill_t(const AttnArgs& a, cudaStream_t st) {
   return cudaGetLastError();
 }
 
-cudaError_t launch_paged_prefill(int type, int head_dim, const AttnArgs& a, cudaStream_t st) {
-#define VTB_PRE(TY) return head_dim == 64 ? launch_prefill_t<TY, 64>(a, st) : launch_prefill_t<TY, 128>(a, st)
-  if (type == F32) VTB_PRE(float);
-  if (type == T_F16) VTB_PRE(__half);
-  VTB_PRE(__nv_bfloat16);
-#undef VTB_PRE
+cudaError_t launch_paged_prefill_f32(int head_dim, const AttnArgs& a, cudaStream_t st) {
+  return head_dim == 64 ? launch_prefill_t<float, 64>(a, st) : launch_prefill_t<float, 128>(a, st);
 }
 
 }  // namespace vtb

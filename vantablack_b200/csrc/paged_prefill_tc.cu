@@ -1,0 +1,454 @@
+// paged_prefill_tc.cu -- chunk attention over the paged cache on the 5th-
+// generation tensor cores, for f16 and bf16 caches.
+//
+// A CTA takes 256 query rows of one kv head (rows = (token, head of the group)
+// pairs in token order, as in paged_prefill_kernel) as two tiles A and B of 128,
+// and walks the positions they see in tiles of 128.  Per tile of positions:
+//   S = Q K^T       tcgen05.mma, both operands K-major in 128-byte-swizzled
+//                   shared tiles, S (f32) in TMEM
+//   P = 2^(S - m)   one thread per row: the row maximum and sum need no
+//                   exchange; P (16 bits) overwrites S in TMEM
+//   O += P V        tcgen05.mma with P from TMEM and V (rows of positions,
+//                   MN-major) from shared memory, O (f32) in TMEM
+// The two tiles alternate: while the tensor cores work on one, eight warps of
+// softmax threads (four per tile) work on the other.  O is rescaled only when
+// a row's maximum has grown by more than 8 (a factor of 256, which both types
+// hold), which after the first tiles hardly ever happens.
+//
+// Warps 0-3: softmax of A; 4-7: of B; warp 8: one thread issues the MMAs; 9-11:
+// gather K and V rows through the page table with cp.async into two stages
+// each.  Rows behind the last position are zeros, so what lies in the rest of
+// a page never meets P = 0.
+//
+// The scale is taken positive (a negative one negates Q in the first product),
+// so the maximum of S is the maximum of the scaled scores.
+#include <type_traits>
+
+#include "paged.cuh"
+
+namespace vtb {
+
+__device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n"
+      ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, int acc) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n"
+      ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(acc) : "memory");
+}
+// MN-major operand in 128-byte-swizzled atoms of 64 values x 8 rows: rows 8 apart
+// lie 1024 bytes apart, the next 64 values `mn` bytes.
+__device__ __forceinline__ uint64_t sw128_desc_mn(uint32_t saddr, uint32_t mn) {
+  return (sw128_desc(saddr) & ~((uint64_t)0x3fff << 16)) | (uint64_t)(mn >> 4) << 16;
+}
+
+#define VTB_R8(v, i) "=r"(v[i]), "=r"(v[i + 1]), "=r"(v[i + 2]), "=r"(v[i + 3]), "=r"(v[i + 4]), "=r"(v[i + 5]), "=r"(v[i + 6]), "=r"(v[i + 7])
+#define VTB_I8(v, i) "r"(v[i]), "r"(v[i + 1]), "r"(v[i + 2]), "r"(v[i + 3]), "r"(v[i + 4]), "r"(v[i + 5]), "r"(v[i + 6]), "r"(v[i + 7])
+__device__ __forceinline__ void tmem_ld32(uint32_t* v, uint32_t addr) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : VTB_R8(v, 0), VTB_R8(v, 8), VTB_R8(v, 16), VTB_R8(v, 24) : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+      ::VTB_I8(v, 0), VTB_I8(v, 8), VTB_I8(v, 16), VTB_I8(v, 24), "r"(addr) : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+constexpr int TQ = 128, TN = 128, TC_THREADS = 384;
+// Registers per thread after the split: softmax warps, MMA and gather warps.
+// setmaxnreg draws on what the CTA was launched with, so the sum of the shares
+// must not pass it (checked before the launch).
+constexpr int REGS_SOFTMAX = 208, REGS_OTHER = 88;
+template <int HD> struct TcPrefill {
+  static constexpr int ATOM = 128 * 128;                // bytes: 128 rows x 64 values
+  static constexpr int TILE = (HD / 64) * ATOM;         // one operand tile
+  static constexpr int SMEM = 6 * TILE + 1024 + 256;    // Q A, Q B, K x 2, V x 2; alignment; barriers
+  static constexpr int SLOT = 2 * TQ * (HD + 2);        // floats of one split's partial result
+};
+
+struct TcBars {
+  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], done;
+  uint32_t tmem;
+};
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(TC_THREADS, 1) paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, int splits) {
+  using C = TcPrefill<HD>;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  TcBars& bar = *reinterpret_cast<TcBars*>(smem + 6 * C::TILE);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  // blockIdx.x = ((row tile from the last, kv head), split): the longest rows start first
+  const int split = blockIdx.x % splits, unit = blockIdx.x / splits, kvh = unit % a.n_kv;
+  const int units = gridDim.x / splits;
+  RowTile rt;
+  if (!row_tile(a, units / a.n_kv - 1 - unit / a.n_kv, 2 * TQ, rt)) return;
+  const int nflat = rt.n * a.group;
+  const bool two = rt.f0 + TQ < nflat;  // tile B has rows
+  const int last = min(rt.f0 + 2 * TQ, nflat) - 1;
+  const Span sp = span_of(max(0, rt.ctx + rt.f0 / a.group), rt.ctx + last / a.group, a.window, a.sinks);
+  // Tiles of positions that this split walks; those of A end with its own last position.
+  const int all = (sp.n + TN - 1) / TN, j0 = (int)((long long)all * split / splits),
+            j1 = (int)((long long)all * (split + 1) / splits);
+  const int pa = rt.ctx + (min(rt.f0 + TQ, nflat) - 1) / a.group;  // A's last position
+  const int na = max(0, min(j1, pa < 0 ? 0 : (pa - sp.w0 + sp.ns + TN) / TN) - j0), nb = two ? j1 - j0 : 0;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&bar.q_full, 256);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&bar.k_full[i], 96);
+      mbar_init(&bar.v_full[i], 96);
+      mbar_init(&bar.k_empty[i], 1);
+      mbar_init(&bar.v_empty[i], 1);
+      mbar_init(&bar.s_full[i], 1);
+      mbar_init(&bar.p_full[i], TQ);
+    }
+    mbar_init(&bar.done, 1);
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&bar.tmem)));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = bar.tmem;
+  const uint32_t sq = smem_u32(smem), sk = sq + 2 * C::TILE, sv = sq + 4 * C::TILE;
+  const int n = max(na, nb);
+
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OTHER));
+    if (warp == 8) {
+      // ---------------- MMA issuer ----------------
+      if (lane == 0) {
+        constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
+        constexpr uint32_t base = (1u << 4) | (fmt << 7) | (fmt << 10) | ((uint32_t)(TQ >> 4) << 24);
+        const uint32_t id_s = base | (a.negate ? 1u << 13 : 0u) | ((uint32_t)(TN >> 3) << 17);
+        constexpr uint32_t id_o = base | (1u << 16) | ((uint32_t)(HD >> 3) << 17);
+        bool ok = true;
+        auto qk = [&](int w, int j) {
+          const uint32_t q = sq + w * C::TILE, k = sk + (j & 1) * C::TILE;
+#pragma unroll
+          for (int kk = 0; kk < HD / 16; ++kk) {
+            const uint32_t off = (kk / 4) * C::ATOM + (kk % 4) * 32;
+            mma_f16_ss(tmem + w * TN, sw128_desc(q + off), sw128_desc(k + off), id_s, kk != 0);
+          }
+          mma_commit(&bar.s_full[w]);
+        };
+        auto pv = [&](int w, int j) {
+          const uint32_t v = sv + (j & 1) * C::TILE;
+#pragma unroll
+          for (int kk = 0; kk < TN / 16; ++kk)
+            mma_f16_ts(tmem + 256 + w * HD, tmem + w * TN + kk * 8, sw128_desc_mn(v + kk * 2048, C::ATOM), id_o, (j | kk) != 0);
+        };
+        auto wait = [&](uint64_t* b, int phase) {
+          if (ok) ok = mbar_wait_bounded(b, phase & 1);
+        };
+        wait(&bar.q_full, 0);
+        if (n > 0) wait(&bar.k_full[0], 0);
+        tc_fence_after();
+        if (ok && na > 0) qk(0, 0);
+        if (ok && nb > 0) qk(1, 0);
+        if (ok && n > 0) mma_commit(&bar.k_empty[0]);
+        for (int j = 0; j < n && ok; ++j) {
+          wait(&bar.v_full[j & 1], j >> 1);
+          if (j + 1 < n) wait(&bar.k_full[(j + 1) & 1], (j + 1) >> 1);
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            const int m = w ? nb : na;
+            if (j >= m) continue;
+            wait(&bar.p_full[w], j);
+            tc_fence_after();
+            if (!ok) break;
+            pv(w, j);
+            if (j + 1 < m) qk(w, j + 1);  // in order behind the product that reads P from the same columns
+          }
+          if (!ok) break;
+          mma_commit(&bar.v_empty[j & 1]);
+          if (j + 1 < n) mma_commit(&bar.k_empty[(j + 1) & 1]);
+        }
+        mma_commit(&bar.done);
+        mbar_wait_bounded(&bar.done, 0);
+      }
+      __syncwarp();
+    } else {
+      // ---------------- K / V gather ----------------
+      constexpr int PIECES = HD / 8, RPW = 32 / PIECES;  // 16-byte pieces per row, rows per warp round
+      const int pc = lane % PIECES, sub = (warp - 9) * RPW + lane / PIECES;
+      const char* hk = a.kv.k + kvh * a.kv.head_stride + pc * 16;
+      const char* hv = a.kv.v + kvh * a.kv.head_stride + pc * 16;
+      const int32_t* table = a.kv.table + rt.s * a.kv.table_stride;
+      auto gather = [&](const char* src, uint32_t dst, int j) {
+        const uint32_t d0 = dst + (pc >> 3) * C::ATOM;
+#pragma unroll 4
+        for (int r = sub; r < TN; r += 3 * RPW) {
+          const int v = (j0 + j) * TN + r;
+          const bool live = v < sp.n;
+          long long off = 0;
+          if (live) {
+            const int pos = sp.pos(v);
+            off = page_row(a.kv, __ldg(table + (pos >> a.kv.page_shift)), pos);
+          }
+          cpa16(d0 + r * 128 + (((pc & 7) ^ (r & 7)) << 4), src + off, live);
+        }
+        cpa_commit();
+      };
+      auto arrive = [&](uint64_t* b) {  // this thread's copies of the oldest group have landed
+        fence_async_smem();
+        mbar_arrive(b);
+      };
+      bool ok = true;
+      // copies run one group ahead of their arrival
+      for (int j = 0; j < n && ok; ++j) {
+        if (j >= 2) ok = mbar_wait_bounded(&bar.k_empty[j & 1], ((j >> 1) - 1) & 1);
+        gather(hk, sk + (j & 1) * C::TILE, j);
+        if (j) {
+          cpa_wait<1>();
+          arrive(&bar.v_full[(j - 1) & 1]);
+          if (j >= 2 && ok) ok = mbar_wait_bounded(&bar.v_empty[j & 1], ((j >> 1) - 1) & 1);
+        }
+        gather(hv, sv + (j & 1) * C::TILE, j);
+        cpa_wait<1>();
+        arrive(&bar.k_full[j & 1]);
+      }
+      cpa_wait<0>();
+      if (n > 0) arrive(&bar.v_full[(n - 1) & 1]);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
+    // ---------------- softmax: one row per thread ----------------
+    const int w = warp >> 2, r = threadIdx.x & 127, f = rt.f0 + w * TQ + r;
+    const bool row = f < nflat;
+    const int head = kvh * a.group + (row ? f % a.group : 0);
+    const long long tok = rt.r0 + (row ? f / a.group : 0);
+    {  // this row of Q into the swizzled tile
+      const uint4* q = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + tok * a.q_row + head * a.q_head);
+      unsigned char* d = smem + w * C::TILE + r * 128;
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c)
+        *reinterpret_cast<uint4*>(d + (c >> 3) * C::ATOM + (((c & 7) ^ (r & 7)) << 4)) = row ? __ldg(q + c) : make_uint4(0, 0, 0, 0);
+      fence_async_smem();
+      mbar_arrive(&bar.q_full);
+    }
+    // The row sees the index ranges [0, va) (sinks) and [vb, vc) of the span.
+    const int p = rt.ctx + f / a.group;
+    int va = 0, vb = 0, vc = sp.n;
+    if (row) {
+      vc = p < 0 ? 0 : p - sp.w0 + sp.ns + 1;
+      if (a.window && p >= 0) {
+        vb = max(0, p + 1 - a.window) - sp.w0 + sp.ns;
+        va = min(a.sinks, vb);
+      }
+    }
+    const int m_tiles = w ? nb : na;
+    const uint32_t ts = tmem + w * TN + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t to = tmem + 256 + w * HD + ((uint32_t)((warp & 3) * 32) << 16);
+    float m = -INFINITY, l = 0.f;  // the maximum that P is relative to (in units of log2), the row's sum
+    bool ok = true;
+    for (int j = 0; j < m_tiles; ++j) {
+      ok = ok && mbar_wait_bounded(&bar.s_full[w], j & 1);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t s[TN];
+#pragma unroll
+      for (int c = 0; c < TN; c += 32) tmem_ld32(s + c, ts + c);
+      tmem_wait_ld();
+      const int v0 = (j0 + j) * TN;
+      if (__any_sync(0xffffffffu, v0 + TN > vc || (v0 < vb && v0 + TN > va))) {
+        const int xa = va - v0, xb = vb - v0, xc = vc - v0;
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+          if (i >= xc || (i < xb && i >= xa)) s[i] = 0xff800000u;
+      }
+      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int i = 0; i < TN; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]));
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale2;
+      if (__any_sync(0xffffffffu, top > m + 8.f)) {
+        const float mn = fmaxf(m, top), k = m == -INFINITY ? 0.f : ex2(m - mn);
+        m = mn;
+        l *= k;
+        if (j > 0) {  // every product so far is complete: S was issued behind them
+#pragma unroll 1
+          for (int c = 0; c < HD; c += 32) {
+            uint32_t o[32];
+            tmem_ld32(o, to + c);
+            tmem_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * k);
+            tmem_st32(to + c, o);
+          }
+        }
+      }
+      const float b = m == -INFINITY ? 0.f : -m;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < TN; i += 2) {
+        const float x = ex2(fmaf(__uint_as_float(s[i]), a.scale2, b)), y = ex2(fmaf(__uint_as_float(s[i + 1]), a.scale2, b));
+        sum[i & 2] += x;
+        sum[(i & 2) + 1] += y;
+        s[i / 2] = pack2<T>(x, y);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      tmem_st32(ts, s);
+      tmem_st32(ts + 32, s + 32);
+      tmem_wait_st();
+      tc_fence_before();
+      mbar_arrive(&bar.p_full[w]);
+    }
+    // ---------------- output ----------------
+    ok = ok && mbar_wait_bounded(&bar.done, 0);
+    if (ok) {
+      tc_fence_after();
+      float* part = a.part + (long long)blockIdx.x * C::SLOT;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      T* out = static_cast<T*>(a.out) + tok * a.o_row + head * a.o_head;
+#pragma unroll 1
+      for (int c = 0; c < HD; c += 32) {
+        uint32_t o[32];
+        if (m_tiles > 0) {
+          tmem_ld32(o, to + c);
+          tmem_wait_ld();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0u;
+        }
+        if (!row) continue;
+        if (splits == 1) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            uint4 x;
+            x.x = pack2<T>(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
+            x.y = pack2<T>(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+            x.z = pack2<T>(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
+            x.w = pack2<T>(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
+            *reinterpret_cast<uint4*>(out + c + i) = x;
+          }
+        } else {
+          float* d = part + 4 * TQ + (long long)(w * TQ + r) * HD + c;
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<float4*>(d + i) = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]),
+                                                            __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+        }
+      }
+      if (splits > 1 && row) {
+        part[w * TQ + r] = m_tiles > 0 ? m : -INFINITY;
+        part[2 * TQ + w * TQ + r] = l;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
+  }
+}
+
+// Adds the splits of 256 rows, 16 rows per CTA: out = sum_i o_i 2^(m_i - M) / sum_i l_i 2^(m_i - M).
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) paged_prefill_join_kernel(const __grid_constant__ AttnArgs a, int splits) {
+  using C = TcPrefill<HD>;
+  const int unit = blockIdx.x >> 4, kvh = unit % a.n_kv, units = gridDim.x >> 4;
+  RowTile rt;
+  const bool any = row_tile(a, units / a.n_kv - 1 - unit / a.n_kv, 2 * TQ, rt);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!any) return;
+  constexpr int LANES = HD / 8;  // threads per row, 8 values each
+  for (int x = threadIdx.x; x < 16 * LANES; x += 256) {
+    const int r = (blockIdx.x & 15) * 16 + x / LANES, c = (x % LANES) * 8, f = rt.f0 + r;
+    if (f >= rt.n * a.group) continue;
+    const float* p = a.part + (long long)unit * splits * C::SLOT;
+    float M = -INFINITY, L = 0.f, acc[8] = {};
+    for (int i = 0; i < splits; ++i) M = fmaxf(M, p[(long long)i * C::SLOT + r]);
+    const float b = M == -INFINITY ? 0.f : M;
+#pragma unroll 4
+    for (int i = 0; i < splits; ++i) {
+      const float* q = p + (long long)i * C::SLOT;
+      const float e = exp2f(q[r] - b);
+      L += q[2 * TQ + r] * e;
+      const float4 u = *reinterpret_cast<const float4*>(q + 4 * TQ + (long long)r * HD + c);
+      const float4 v = *reinterpret_cast<const float4*>(q + 4 * TQ + (long long)r * HD + c + 4);
+      acc[0] += u.x * e; acc[1] += u.y * e; acc[2] += u.z * e; acc[3] += u.w * e;
+      acc[4] += v.x * e; acc[5] += v.y * e; acc[6] += v.z * e; acc[7] += v.w * e;
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) acc[i] *= inv;
+    store_vec(static_cast<T*>(a.out) + (rt.r0 + f / a.group) * a.o_row + (long long)(kvh * a.group + f % a.group) * a.o_head + c, acc);
+  }
+}
+
+// CTAs that a call of few row tiles spreads over: one per SM.
+size_t paged_prefill_tc_workspace(int head_dim) {
+  return (size_t)sm_count(current_device()) * 2 * TQ * (head_dim + 2) * sizeof(float);
+}
+
+// Whether the kernel was built with the registers that its split adds up to.
+template <auto KERN>
+static cudaError_t check_register_split(int dev) {
+  static std::atomic<int> known[VTB_MAX_DEVICES];
+  if (known[dev].load(std::memory_order_relaxed)) return cudaSuccess;
+  cudaFuncAttributes f;
+  const cudaError_t e = cudaFuncGetAttributes(&f, KERN);
+  if (e) return e;
+  if (f.numRegs / 8 * 8 * TC_THREADS < 256 * REGS_SOFTMAX + 128 * REGS_OTHER) return cudaErrorInvalidConfiguration;
+  known[dev].store(1, std::memory_order_relaxed);
+  return cudaSuccess;
+}
+
+template <typename T, int HD>
+static cudaError_t launch_prefill_tc_t(AttnArgs a, cudaStream_t st) {
+  using C = TcPrefill<HD>;
+  a.negate = a.scale2 < 0.f;
+  a.scale2 = fmaxf(fabsf(a.scale2), 1e-36f);  // not 0: masked scores have to stay -inf
+  const int dev = current_device();
+  cudaError_t e = ensure_smem_attr<paged_prefill_tc_kernel<T, HD>>(dev, C::SMEM);
+  if (e || (e = check_register_split<paged_prefill_tc_kernel<T, HD>>(dev))) return e;
+  const long long units = ((long long)a.rows * a.group / (2 * TQ) + a.kv.n_seqs) * a.n_kv;
+  if (units > 0x7fffffffll / 16) return cudaErrorInvalidValue;
+  // Fewer row tiles than SMs: the positions are split too, down to two tiles of
+  // positions per CTA (below that the join costs more than the split gives).
+  const long long cap = (long long)a.kv.pages_per_seq << a.kv.page_shift;
+  long long seen = a.window ? (long long)a.window + a.sinks + a.rows : cap;
+  if (seen > cap) seen = cap;
+  long long splits = sm_count(dev) / units, most = seen / (2 * TN);
+  if (splits > most) splits = most;
+  if (splits < 1) splits = 1;
+  paged_prefill_tc_kernel<T, HD><<<(unsigned)(units * splits), TC_THREADS, C::SMEM, st>>>(a, (int)splits);
+  if ((e = cudaGetLastError()) || splits == 1) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(units * 16));
+  cfg.blockDim = dim3(256);
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_prefill_join_kernel<T, HD>, a, (int)splits);
+}
+
+cudaError_t launch_paged_prefill_tc(int type, int head_dim, const AttnArgs& a, cudaStream_t st) {
+  if (type == T_F16) return head_dim == 64 ? launch_prefill_tc_t<__half, 64>(a, st) : launch_prefill_tc_t<__half, 128>(a, st);
+  return head_dim == 64 ? launch_prefill_tc_t<__nv_bfloat16, 64>(a, st) : launch_prefill_tc_t<__nv_bfloat16, 128>(a, st);
+}
+
+}  // namespace vtb

@@ -7,6 +7,7 @@ tensors are flat ``torch.uint8`` CUDA tensors of packed GGUF blocks.
 from __future__ import annotations
 
 import ctypes as C
+import struct
 
 import torch
 
@@ -147,50 +148,73 @@ def gemm(quant: int, w: torch.Tensor, acts: torch.Tensor, m: int, k: int, precis
 
 
 # ---- paged key-value cache ----
+# A decode step makes these calls once per layer, so the host side is kept short: descriptors are packed as bytes
+# (struct, in the C layouts of _lib.PagedKv / PagedRows / PagedAttn), device and stream are read as plain integers.
 
 KV_TYPES = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+_KV = struct.Struct("@2P4i4qPq2i")
+_ROWS = struct.Struct("@2iq3P6q2Pq2P")
+_ATTN = struct.Struct("@2P4q3if2PN")
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def _on(dev: torch.device, t: torch.Tensor, name: str, dtype: torch.dtype) -> None:
-    if t.device != dev:
-        raise ValueError(f"{name} must be on {dev}, as the cache is")
-    if t.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype}")
+def _stream_of(dev: int) -> int:
+    return _raw_stream(dev) if _raw_stream is not None else _stream()
 
 
-def _paged_kv(k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor | None) -> _lib.PagedKv:
+def _on(dev: int, dtype: torch.dtype, **tensors) -> None:
+    for name, t in tensors.items():
+        if t.get_device() != dev:
+            raise ValueError(f"{name} must be on the cache's device")
+        if t.dtype is not dtype:
+            raise ValueError(f"{name} must be {dtype}")
+
+
+def _paged_kv(k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor | None):
     """The cache as the C ABI describes it; k, v [n_pages, n_kv_heads, page_size, head_dim]
-    (any order of strides, so a [page, slot, head, dim] cache goes in as .transpose(1, 2))."""
-    if not k.is_cuda or k.device.index != torch.cuda.current_device():
+    (any order of strides, so a [page, slot, head, dim] cache goes in as .transpose(1, 2)).
+    Returns (descriptor, device index, dtype, shape, n_seqs)."""
+    dev, dt, st, shape = k.get_device(), k.dtype, k.stride(), k.shape
+    if dev < 0 or dev != torch.cuda.current_device():
         raise ValueError("the cache must be on the current CUDA device")
-    st = k.stride()
-    if k.dim() != 4 or st[3] != 1 or k.dtype not in KV_TYPES:
+    if len(st) != 4 or st[3] != 1 or dt not in KV_TYPES:
         raise ValueError("the cache is [n_pages, n_kv_heads, page_size, head_dim], f32, f16 or bf16, dense in head_dim")
-    _on(k.device, v, "v", k.dtype)
-    if v.shape != k.shape or v.stride() != st:
-        raise ValueError("k and v must agree in shape and strides")
-    n_pages, n_kv, page_size, hd = k.shape
+    if v.get_device() != dev or v.dtype is not dt or v.stride() != st or v.shape != shape:
+        raise ValueError("k and v must agree in device, type, shape and strides")
+    n_pages, n_kv, page_size, hd = shape
     if page_table is None:
-        return _lib.PagedKv(k.data_ptr(), v.data_ptr(), KV_TYPES[k.dtype], n_kv, hd, page_size, n_pages, st[0], st[1],
-                            st[2], None, 0, 0, 0)
-    _on(k.device, page_table, "page_table", torch.int32)
-    if page_table.dim() != 2 or (page_table.stride(1) != 1 and page_table.shape[1] > 1):
-        raise ValueError("page_table is [n_seqs, pages per sequence], dense in its rows")
-    n, per = page_table.shape
-    ld = page_table.stride(0)
-    return _lib.PagedKv(k.data_ptr(), v.data_ptr(), KV_TYPES[k.dtype], n_kv, hd, page_size, n_pages, st[0], st[1],
-                        st[2], page_table.data_ptr(), ld if n > 1 else max(ld, per), n, per)
+        table = (0, 0, 0, 0)
+    else:
+        _on(dev, torch.int32, page_table=page_table)
+        if page_table.dim() != 2:
+            raise ValueError("page_table is [n_seqs, pages per sequence]")
+        (n, per), (ld, one) = page_table.shape, page_table.stride()
+        if one != 1 and per > 1:
+            raise ValueError("page_table must be dense in its rows")
+        table = (page_table.data_ptr(), ld if n > 1 else max(ld, per), n, per)
+    kv = _KV.pack(k.data_ptr(), v.data_ptr(), KV_TYPES[dt], n_kv, hd, page_size, n_pages, st[0], st[1], st[2], *table)
+    return kv, dev, dt, shape, table[2]
 
 
-def _rows(x: torch.Tensor, name: str, dev: torch.device, dtype: torch.dtype, heads: int | None, hd: int):
+def _rows(x: torch.Tensor, name: str, dev: int, dtype: torch.dtype, heads: int | None, hd: int):
     """(row stride, head stride) of [rows, heads, head_dim] rows."""
-    _on(dev, x, name, dtype)
-    if x.dim() != 3 or x.shape[2] != hd or (heads is not None and x.shape[1] != heads):
-        raise ValueError(f"{name} has the wrong shape {tuple(x.shape)}")
-    st = x.stride()
+    st, shape = x.stride(), x.shape
+    if x.get_device() != dev or x.dtype is not dtype:
+        _on(dev, dtype, **{name: x})
+    if len(st) != 3 or shape[2] != hd or (heads is not None and shape[1] != heads):
+        raise ValueError(f"{name} has the wrong shape {tuple(shape)}")
     if st[2] != 1:
         raise ValueError(f"{name} must be dense in head_dim")
-    return st[0], st[1] if x.shape[1] > 1 else hd
+    return st[0], st[1] if shape[1] > 1 else hd
+
+
+def _vec(x: torch.Tensor, name: str, dev: int, n: int) -> int:
+    """Address of a contiguous int32 list of n entries."""
+    if x.get_device() != dev or x.dtype is not torch.int32:
+        _on(dev, torch.int32, **{name: x})
+    if x.dim() != 1 or x.numel() != n or (n > 1 and x.stride(0) != 1):
+        raise ValueError(f"{name} must be a contiguous list of {n} entries")
+    return x.data_ptr()
 
 
 def paged_append(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor, k: torch.Tensor,
@@ -199,40 +223,40 @@ def paged_append(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch
     """Writes the rows k, v [rows, n_kv_heads, head_dim] (f32 or the cache's type) into the pages at position
     pos[r] of sequence seq[r] (int32; a negative one skips the row), rotated by rope [positions, head_dim] if
     given; with q [rows, n_heads, head_dim] also returns the rotated queries in the cache's type (in q_out)."""
-    kv = _paged_kv(k_pages, v_pages, page_table)
-    dev, n_kv, hd = k_pages.device, kv.n_kv_heads, kv.head_dim
-    x = k.dtype
-    if x not in (torch.float32, k_pages.dtype):
+    kv, dev, dt, shape, _ = _paged_kv(k_pages, v_pages, page_table)
+    n_kv, hd, x = shape[1], shape[3], k.dtype
+    if x is not torch.float32 and x is not dt:
         raise ValueError("rows must be f32 or of the cache's type")
     ks = _rows(k, "k", dev, x, n_kv, hd)
     vs = _rows(v, "v", dev, x, n_kv, hd)
     n = k.shape[0]
-    _on(dev, seq, "seq", torch.int32); _on(dev, pos, "pos", torch.int32)
-    if v.shape[0] != n or seq.shape != (n,) or pos.shape != (n,) or not (seq.is_contiguous() and pos.is_contiguous()):
-        raise ValueError("k, v, seq and pos must have one entry per row")
-    qs, heads = (0, 0), 0
+    if v.shape[0] != n:
+        raise ValueError("v must have one entry per row")
+    at = (_vec(seq, "seq", dev, n), _vec(pos, "pos", dev, n))
+    qs, heads, q_ptr, o_ptr = (0, 0), 0, 0, 0
     if q is not None:
         qs, heads = _rows(q, "q", dev, x, None, hd), q.shape[1]
         if q.shape[0] != n:
             raise ValueError("q must have one entry per row")
         if q_out is None:
-            q_out = torch.empty(n, heads, hd, dtype=k_pages.dtype, device=dev)
-        _on(dev, q_out, "q_out", k_pages.dtype)
-        if q_out.shape != (n, heads, hd) or not q_out.is_contiguous():
-            raise ValueError("q_out must be contiguous [rows, n_heads, head_dim]")
+            q_out = torch.empty(n, heads, hd, dtype=dt, device=k_pages.device)
+        else:
+            _rows(q_out, "q_out", dev, dt, heads, hd)
+            if q_out.shape[0] != n or not q_out.is_contiguous():
+                raise ValueError("q_out must be contiguous [rows, n_heads, head_dim]")
+        q_ptr, o_ptr = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out without q")
+    turn = (0, 0)
     if rope is not None:
-        _on(dev, rope, "rope", torch.float32)
+        _on(dev, torch.float32, rope=rope)
         if rope.dim() != 2 or rope.shape[1] != hd or not rope.is_contiguous():
             raise ValueError("rope must be contiguous f32 [positions, head_dim]")
+        turn = (rope.data_ptr(), rope.shape[0])
     if n == 0:
         return q_out
-    r = _lib.PagedRows(KV_TYPES[x], heads, n, k.data_ptr(), v.data_ptr(), q.data_ptr() if q is not None else None,
-                       *ks, *vs, *qs, q_out.data_ptr() if q is not None else None,
-                       rope.data_ptr() if rope is not None else None, rope.shape[0] if rope is not None else 0,
-                       seq.data_ptr(), pos.data_ptr())
-    _lib.check(lib.vtb_cuda_paged_append(C.byref(kv), C.byref(r), _stream()), "vtb_cuda_paged_append")
+    r = _ROWS.pack(KV_TYPES[x], heads, n, k.data_ptr(), v.data_ptr(), q_ptr, *ks, *vs, *qs, o_ptr, *turn, *at)
+    _lib.check(lib.vtb_cuda_paged_append(kv, r, _stream_of(dev)), "vtb_cuda_paged_append")
     return q_out
 
 
@@ -243,22 +267,21 @@ def paged_attention_workspace(dtype: torch.dtype, n_heads: int, n_kv_heads: int,
     return torch.empty(n, dtype=torch.uint8, device=device)
 
 
-def _attn(kv, q, k_pages, lens, scale, window, sinks, out, workspace):
-    dev, hd = k_pages.device, kv.head_dim
-    qs = _rows(q, "q", dev, k_pages.dtype, None, hd)
+def _attn(q, k_pages, dev, dt, shape, n_seqs, lens, scale, window, sinks, out, workspace):
+    n_kv, hd = shape[1], shape[3]
+    qs, heads = _rows(q, "q", dev, dt, None, hd), q.shape[1]
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    os = _rows(out, "out", dev, k_pages.dtype, q.shape[1], hd)
-    _on(dev, lens, "lens", torch.int32)
-    if out.shape != q.shape or lens.shape != (kv.n_seqs,) or not lens.is_contiguous():
-        raise ValueError("out must have q's shape, lens one entry per sequence")
+        out = torch.empty(q.shape, dtype=dt, device=k_pages.device)
+    os = _rows(out, "out", dev, dt, heads, hd)
+    if out.shape[0] != q.shape[0]:
+        raise ValueError("out must have q's shape")
     if workspace is None:
-        workspace = paged_attention_workspace(k_pages.dtype, q.shape[1], kv.n_kv_heads, hd, dev)
-    _on(dev, workspace, "workspace", torch.uint8)
-    if scale is None:
-        scale = hd ** -0.5
-    return out, _lib.PagedAttn(q.data_ptr(), out.data_ptr(), *qs, *os, q.shape[1], window, sinks, scale,
-                               lens.data_ptr(), workspace.data_ptr(), workspace.numel()), workspace
+        workspace = paged_attention_workspace(dt, heads, n_kv, hd, k_pages.device)
+    elif workspace.get_device() != dev or workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous uint8 tensor on the cache's device")
+    a = _ATTN.pack(q.data_ptr(), out.data_ptr(), *qs, *os, heads, window, sinks, hd ** -0.5 if scale is None else scale,
+                   _vec(lens, "lens", dev, n_seqs), workspace.data_ptr(), workspace.numel())
+    return out, a, workspace
 
 
 def paged_attention_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -267,11 +290,11 @@ def paged_attention_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     """Attention of one new token per sequence, q [n_seqs, n_heads, head_dim] at position lens[s] - 1, over the
     sequence's pages.  window > 0: the last `window` positions and the first `sinks` are visible.  scale: 1 / sqrt(head_dim)
     unless given.  A sequence of length 0 gives zeros."""
-    kv = _paged_kv(k_pages, v_pages, page_table)
-    if q.shape[0] != kv.n_seqs:
+    kv, dev, dt, shape, n_seqs = _paged_kv(k_pages, v_pages, page_table)
+    if q.shape[0] != n_seqs:
         raise ValueError("q must have one row per sequence")
-    out, a, workspace = _attn(kv, q, k_pages, lens, scale, window, sinks, out, workspace)
-    _lib.check(lib.vtb_cuda_paged_attn_decode(C.byref(kv), C.byref(a), _stream()), "vtb_cuda_paged_attn_decode")
+    out, a, workspace = _attn(q, k_pages, dev, dt, shape, n_seqs, lens, scale, window, sinks, out, workspace)
+    _lib.check(lib.vtb_cuda_paged_attn_decode(kv, a, _stream_of(dev)), "vtb_cuda_paged_attn_decode")
     return out
 
 
@@ -282,13 +305,10 @@ def paged_attention_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     """Causal attention of a chunk of new tokens per sequence: rows starts[s] .. starts[s + 1] of q
     [rows, n_heads, head_dim] are the last tokens of sequence s's lens[s] positions, whose keys and values are
     in the pages already (paged_append).  Rows that no sequence holds are left as they were."""
-    kv = _paged_kv(k_pages, v_pages, page_table)
-    _on(k_pages.device, starts, "starts", torch.int32)
-    if starts.shape != (kv.n_seqs + 1,) or not starts.is_contiguous():
-        raise ValueError("starts must have one entry per sequence and one more")
-    out, a, workspace = _attn(kv, q, k_pages, lens, scale, window, sinks, out, workspace)
-    _lib.check(lib.vtb_cuda_paged_attn_prefill(C.byref(kv), C.byref(a), starts.data_ptr(), q.shape[0], _stream()),
-               "vtb_cuda_paged_attn_prefill")
+    kv, dev, dt, shape, n_seqs = _paged_kv(k_pages, v_pages, page_table)
+    at = _vec(starts, "starts", dev, n_seqs + 1)
+    out, a, workspace = _attn(q, k_pages, dev, dt, shape, n_seqs, lens, scale, window, sinks, out, workspace)
+    _lib.check(lib.vtb_cuda_paged_attn_prefill(kv, a, at, q.shape[0], _stream_of(dev)), "vtb_cuda_paged_attn_prefill")
     return out
 
 
@@ -302,19 +322,11 @@ def paged_copy(k_cache: torch.Tensor, v_cache: torch.Tensor, src: torch.Tensor, 
         raise ValueError("the cache is [n_layers, n_pages, n_kv_heads, page_size, head_dim], k and v alike")
     if (page_table is None) != (page_map is None):
         raise ValueError("page_table and page_map go together")
-    kv = _paged_kv(k_cache[0], v_cache[0], page_table)
-    dev, n = k_cache.device, src.numel()
-    for t, nm in ((src, "src"), (dst, "dst")):
-        _on(dev, t, nm, torch.int32)
-        if t.shape != (n,) or not t.is_contiguous():
-            raise ValueError("src and dst must be contiguous lists of the same length")
-    if page_map is not None:
-        _on(dev, page_map, "page_map", torch.int32)
-        if page_map.shape != (kv.n_pages,) or not page_map.is_contiguous():
-            raise ValueError("page_map must have one entry per page")
-    _lib.check(lib.vtb_cuda_paged_copy(C.byref(kv), k_cache.shape[0], k_cache.stride(0), src.data_ptr(), dst.data_ptr(), n,
-                                       page_table.data_ptr() if page_table is not None else None,
-                                       page_map.data_ptr() if page_map is not None else None, _stream()),
+    kv, dev, _, shape, _ = _paged_kv(k_cache[0], v_cache[0], page_table)
+    n = src.numel()
+    moves = (_vec(src, "src", dev, n), _vec(dst, "dst", dev, n), n)
+    tables = (page_table.data_ptr(), _vec(page_map, "page_map", dev, shape[0])) if page_map is not None else (0, 0)
+    _lib.check(lib.vtb_cuda_paged_copy(kv, k_cache.shape[0], k_cache.stride(0), *moves, *tables, _stream_of(dev)),
                "vtb_cuda_paged_copy")
 
 
