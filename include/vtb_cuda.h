@@ -176,7 +176,8 @@ int vtb_cuda_gemv_q8_0_q8_0_noalloc(const void *w, const float *x, float *y, int
  * and the same in v.  Any order of the three strides works; [page][head][slot]
  * keeps a head's positions together, which reads fastest.  k, v and every
  * stride in bytes are multiples of 16; page_size is a power of two up to 1024;
- * head_dim is 64 or 128; type is F32, F16 or BF16.
+ * head_dim is 64 or 128; type is F32, F16 or BF16; a table row covers at most
+ * 2^30 positions.
  *
  * Page ids are read only where a position is written or visible, so entries of
  * unused or evicted pages may hold anything (-1).  An id outside [0, n_pages)

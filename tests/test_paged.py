@@ -44,7 +44,7 @@ BAD_KV = [(dict(k=None), -1), (dict(type=8), -8), (dict(head_dim=80), -8), (dict
           (dict(page_size=2048), -1), (dict(n_kv_heads=0), -1), (dict(n_pages=0), -1), (dict(n_pages=1 << 31), -1),
           (dict(page_stride=-8), -1), (dict(slot_stride=65), -1), (dict(head_stride=1 << 50), -1)]
 BAD_TABLE = [(dict(page_table=None), -1), (dict(n_seqs=0), -1), (dict(pages_per_seq=0), -1), (dict(table_stride=2), -1),
-             (dict(pages_per_seq=1 << 30, table_stride=1 << 30), -1)]
+             (dict(pages_per_seq=(1 << 26) + 1, table_stride=1 << 30), -1)]
 
 
 @pytest.mark.parametrize("bad,status", BAD_KV + BAD_TABLE)

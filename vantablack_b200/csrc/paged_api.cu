@@ -23,7 +23,7 @@ static int paged_view(const VtbCudaPagedKv* kv, bool need_table, PagedView* out)
     if (s < 0 || s > (int64_t(1) << 40) || !mul16(s, es))
       return set_err(VTB_CUDA_ERR_INVALID_ARG, "cache strides must be whole numbers of 16 bytes");
   if (need_table && (!kv->page_table || kv->n_seqs < 1 || kv->pages_per_seq < 1 || kv->table_stride < kv->pages_per_seq ||
-                     (int64_t(kv->pages_per_seq) << shift) > INT_MAX))
+                     (int64_t(kv->pages_per_seq) << shift) > (1 << 30)))
     return set_err(VTB_CUDA_ERR_INVALID_ARG, "bad page table");
   *out = PagedView{static_cast<const char*>(kv->k), static_cast<const char*>(kv->v), kv->page_stride * es,
                    kv->head_stride * es, kv->slot_stride * es, kv->page_table, kv->table_stride,

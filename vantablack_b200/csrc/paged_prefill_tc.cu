@@ -15,19 +15,27 @@
 // a row's maximum has grown by more than 8 (a factor of 256, which both types
 // hold), which after the first tiles hardly ever happens.
 //
-// Warps 0-3: softmax of A; 4-7: of B; warp 8: one thread issues the MMAs; 9-11:
-// gather K and V rows through the page table with cp.async into two stages
-// each.  Rows behind the last position are zeros, so what lies in the rest of
-// a page never meets P = 0.
+// Warps 0-3: softmax of A; 4-7: of B; warp 8: one thread issues the MMAs; 9-11
+// bring K and V into two stages each: a tile that some row sees whole comes by
+// TMA, one box per page and 64 values (4-d map over the page pool); a tile at an
+// edge (the last positions, the window's start, the sinks' end, pages of fewer
+// than 8 positions) is gathered row by row with cp.async, zeros in place of
+// positions that no row sees, so what lies in the rest of a page never meets P = 0.
 //
 // The scale is taken positive (a negative one negates Q in the first product),
 // so the maximum of S is the maximum of the scaled scores.
 #include <type_traits>
 
 #include "paged.cuh"
+#include "tma.cuh"
 
 namespace vtb {
 
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, int w, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar)) : "memory");
+}
 __device__ __forceinline__ void mma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int acc) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
@@ -86,7 +94,9 @@ struct TcBars {
 };
 
 template <typename T, int HD>
-__global__ void __launch_bounds__(TC_THREADS, 1) paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, int splits) {
+__global__ void __launch_bounds__(TC_THREADS, 1)
+paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constant__ CUtensorMap map_k,
+                        const __grid_constant__ CUtensorMap map_v, int splits, int box) {
   using C = TcPrefill<HD>;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -101,18 +111,23 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_prefill_tc_kernel(const _
   const int nflat = rt.n * a.group;
   const bool two = rt.f0 + TQ < nflat;  // tile B has rows
   const int last = min(rt.f0 + 2 * TQ, nflat) - 1;
-  const Span sp = span_of(max(0, rt.ctx + rt.f0 / a.group), rt.ctx + last / a.group, a.window, a.sinks);
-  // Tiles of positions that this split walks; those of A end with its own last position.
-  const int all = (sp.n + TN - 1) / TN, j0 = (int)((long long)all * split / splits),
-            j1 = (int)((long long)all * (split + 1) / splits);
+  // Positions [w0, p1] and, when a window has left them behind, the first `sinks`
+  // of [0, w0), in tiles at multiples of TN: `ks` sink tiles, then those from kw.
+  const int p1 = rt.ctx + last / a.group, p0 = max(0, rt.ctx + rt.f0 / a.group);
+  const int w0 = a.window && p0 >= a.window ? p0 + 1 - a.window : 0;
+  const int kw0 = w0 / TN, ks = min((min(a.sinks, w0) + TN - 1) / TN, kw0), ke = p1 < 0 ? 0 : p1 / TN + 1;
+  const int kw = ke > 0 ? kw0 : 0, all = p1 < 0 ? 0 : ks + ke - kw;
+  // Tiles that this split walks; those of A end with its own last position.
+  const int j0 = (int)((long long)all * split / splits), j1 = (int)((long long)all * (split + 1) / splits);
   const int pa = rt.ctx + (min(rt.f0 + TQ, nflat) - 1) / a.group;  // A's last position
-  const int na = max(0, min(j1, pa < 0 ? 0 : (pa - sp.w0 + sp.ns + TN) / TN) - j0), nb = two ? j1 - j0 : 0;
+  const int na = max(0, min(j1, pa < 0 ? 0 : ks + pa / TN + 1 - kw) - j0), nb = two ? j1 - j0 : 0;
+  auto tile_pos = [&](int j) { return (j0 + j < ks ? j0 + j : j0 + j - ks + kw) * TN; };  // first position of tile j
 
   if (threadIdx.x == 0) {
     mbar_init(&bar.q_full, 256);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar.k_full[i], 96);
-      mbar_init(&bar.v_full[i], 96);
+      mbar_init(&bar.k_full[i], 3);  // the three gather warps
+      mbar_init(&bar.v_full[i], 3);
       mbar_init(&bar.k_empty[i], 1);
       mbar_init(&bar.v_empty[i], 1);
       mbar_init(&bar.s_full[i], 1);
@@ -188,47 +203,70 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_prefill_tc_kernel(const _
       }
       __syncwarp();
     } else {
-      // ---------------- K / V gather ----------------
-      constexpr int PIECES = HD / 8, RPW = 32 / PIECES;  // 16-byte pieces per row, rows per warp round
-      const int pc = lane % PIECES, sub = (warp - 9) * RPW + lane / PIECES;
-      const char* hk = a.kv.k + kvh * a.kv.head_stride + pc * 16;
-      const char* hv = a.kv.v + kvh * a.kv.head_stride + pc * 16;
+      // ---------------- K / V tiles ----------------
       const int32_t* table = a.kv.table + rt.s * a.kv.table_stride;
-      auto gather = [&](const char* src, uint32_t dst, int j) {
+      // by TMA: lane i of warp 9 loads box i (page i / atoms, atom i % atoms)
+      auto boxes = [&](const CUtensorMap* map, uint32_t dst, int t0, uint64_t* full) {
+        if (warp == 9) {
+          constexpr int ATOMS = HD / 64;
+          const int i = lane / ATOMS, at = lane % ATOMS;
+          if (lane == 0) mbar_expect_tx(full, C::TILE);
+          __syncwarp();
+          if (i * box < TN) {
+            const int pos = t0 + i * box;
+            int page = __ldg(table + (pos >> a.kv.page_shift));
+            if ((unsigned)page >= (unsigned)a.kv.n_pages) {
+              flag_error(DEV_ERR_BAD_ARG);
+              page = 0;
+            }
+            tma_load_4d(dst + at * C::ATOM + i * box * 128, map, at * 64, pos & ((1 << a.kv.page_shift) - 1), kvh, page, full);
+          }
+        } else if (lane == 0) {
+          mbar_arrive(full);
+        }
+      };
+      // by rows: 16-byte pieces, PIECES lanes to a row
+      constexpr int PIECES = HD / 8, RPW = 32 / PIECES;
+      const int pc = lane % PIECES, sub = (warp - 9) * RPW + lane / PIECES;
+      auto rows = [&](const char* base, uint32_t dst, int t0) {
+        const char* src = base + kvh * a.kv.head_stride + pc * 16;
         const uint32_t d0 = dst + (pc >> 3) * C::ATOM;
 #pragma unroll 4
         for (int r = sub; r < TN; r += 3 * RPW) {
-          const int v = (j0 + j) * TN + r;
-          const bool live = v < sp.n;
-          long long off = 0;
-          if (live) {
-            const int pos = sp.pos(v);
-            off = page_row(a.kv, __ldg(table + (pos >> a.kv.page_shift)), pos);
-          }
+          const int pos = t0 + r;
+          const bool live = pos <= p1 && (pos >= w0 || pos < a.sinks);
+          const long long off = live ? page_row(a.kv, __ldg(table + (pos >> a.kv.page_shift)), pos) : 0;
           cpa16(d0 + r * 128 + (((pc & 7) ^ (r & 7)) << 4), src + off, live);
         }
         cpa_commit();
       };
-      auto arrive = [&](uint64_t* b) {  // this thread's copies of the oldest group have landed
+      auto landed = [&](uint64_t* full) {  // this warp's copies are in shared memory
         fence_async_smem();
-        mbar_arrive(b);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full);
       };
       bool ok = true;
-      // copies run one group ahead of their arrival
       for (int j = 0; j < n && ok; ++j) {
-        if (j >= 2) ok = mbar_wait_bounded(&bar.k_empty[j & 1], ((j >> 1) - 1) & 1);
-        gather(hk, sk + (j & 1) * C::TILE, j);
-        if (j) {
+        const int t0 = tile_pos(j), i = j & 1;
+        const bool edge = !box || t0 + TN > p1 + 1 || (t0 < w0 && t0 + TN > a.sinks);
+        const uint32_t dk = sk + i * C::TILE, dv = sv + i * C::TILE;
+        if (j >= 2) ok = mbar_wait_bounded(&bar.k_empty[i], ((j >> 1) - 1) & 1);
+        if (!ok) break;
+        if (edge) rows(a.kv.k, dk, t0);
+        else boxes(&map_k, dk, t0, &bar.k_full[i]);
+        if (j >= 2) ok = mbar_wait_bounded(&bar.v_empty[i], ((j >> 1) - 1) & 1);
+        if (!ok) break;
+        if (edge) {
+          rows(a.kv.v, dv, t0);
           cpa_wait<1>();
-          arrive(&bar.v_full[(j - 1) & 1]);
-          if (j >= 2 && ok) ok = mbar_wait_bounded(&bar.v_empty[j & 1], ((j >> 1) - 1) & 1);
+          landed(&bar.k_full[i]);
+          cpa_wait<0>();
+          landed(&bar.v_full[i]);
+        } else {
+          boxes(&map_v, dv, t0, &bar.v_full[i]);
         }
-        gather(hv, sv + (j & 1) * C::TILE, j);
-        cpa_wait<1>();
-        arrive(&bar.k_full[j & 1]);
       }
       cpa_wait<0>();
-      if (n > 0) arrive(&bar.v_full[(n - 1) & 1]);
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS_SOFTMAX));
@@ -246,14 +284,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_prefill_tc_kernel(const _
       fence_async_smem();
       mbar_arrive(&bar.q_full);
     }
-    // The row sees the index ranges [0, va) (sinks) and [vb, vc) of the span.
+    // The row sees positions [0, va) (sinks) and [vb, vc).
     const int p = rt.ctx + f / a.group;
-    int va = 0, vb = 0, vc = sp.n;
+    int va = 0, vb = 0, vc = 0x7fffffff;
     if (row) {
-      vc = p < 0 ? 0 : p - sp.w0 + sp.ns + 1;
-      if (a.window && p >= 0) {
-        vb = max(0, p + 1 - a.window) - sp.w0 + sp.ns;
-        va = min(a.sinks, vb);
+      vc = p + 1;
+      if (a.window) {
+        vb = vc - a.window;
+        va = a.sinks;
       }
     }
     const int m_tiles = w ? nb : na;
@@ -269,7 +307,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) paged_prefill_tc_kernel(const _
 #pragma unroll
       for (int c = 0; c < TN; c += 32) tmem_ld32(s + c, ts + c);
       tmem_wait_ld();
-      const int v0 = (j0 + j) * TN;
+      const int v0 = tile_pos(j);
       if (__any_sync(0xffffffffu, v0 + TN > vc || (v0 < vb && v0 + TN > va))) {
         const int xa = va - v0, xb = vb - v0, xc = vc - v0;
 #pragma unroll
@@ -401,6 +439,18 @@ size_t paged_prefill_tc_workspace(int head_dim) {
   return (size_t)sm_count(current_device()) * 2 * TQ * (head_dim + 2) * sizeof(float);
 }
 
+// TMA map of a page pool, (value, slot, head, page), in boxes of 64 values x `fit` slots.
+static bool page_map(CUtensorMap* map, const PagedView& kv, const char* base, bool half, int hd, int n_kv, int fit) {
+  auto fn = tmap_encode_fn();
+  if (!fn || !kv.page_stride || !kv.head_stride || !kv.slot_stride || kv.page_stride >= (1ll << 40)) return false;
+  const cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)1 << kv.page_shift, (cuuint64_t)n_kv, (cuuint64_t)kv.n_pages};
+  const cuuint64_t strides[3] = {(cuuint64_t)kv.slot_stride, (cuuint64_t)kv.head_stride, (cuuint64_t)kv.page_stride};
+  const cuuint32_t boxes[4] = {64, (cuuint32_t)fit, 1, 1}, ones[4] = {1, 1, 1, 1};
+  return fn(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<char*>(base), dims,
+            strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Whether the kernel was built with the registers that its split adds up to.
 template <auto KERN>
 static cudaError_t check_register_split(int dev) {
@@ -432,7 +482,11 @@ static cudaError_t launch_prefill_tc_t(AttnArgs a, cudaStream_t st) {
   long long splits = sm_count(dev) / units, most = seen / (2 * TN);
   if (splits > most) splits = most;
   if (splits < 1) splits = 1;
-  paged_prefill_tc_kernel<T, HD><<<(unsigned)(units * splits), TC_THREADS, C::SMEM, st>>>(a, (int)splits);
+  CUtensorMap map_k = {}, map_v = {};
+  const int slots = 1 << a.kv.page_shift, fit = slots < TN ? slots : TN;
+  const int box = slots >= 8 && page_map(&map_k, a.kv, a.kv.k, std::is_same<T, __half>::value, HD, a.n_kv, fit) &&
+                          page_map(&map_v, a.kv, a.kv.v, std::is_same<T, __half>::value, HD, a.n_kv, fit) ? fit : 0;
+  paged_prefill_tc_kernel<T, HD><<<(unsigned)(units * splits), TC_THREADS, C::SMEM, st>>>(a, map_k, map_v, (int)splits, box);
   if ((e = cudaGetLastError()) || splits == 1) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units * 16));
