@@ -359,8 +359,11 @@ __device__ __forceinline__ bool row_tile(const AttnArgs& a, int idx, int tile, R
   const int lane = threadIdx.x & 31;
   long long before = 0;
   for (int s0 = 0; s0 < a.kv.n_seqs; s0 += 32) {
-    int r0 = 0, n = 0;
-    if (s0 + lane < a.kv.n_seqs) n = chunk_rows(a, s0 + lane, r0);
+    int r0 = 0, n = 0, len = 0;
+    if (s0 + lane < a.kv.n_seqs) {
+      len = paged_len(a.kv, a.lens, s0 + lane);
+      n = chunk_rows(a, s0 + lane, r0);
+    }
     const long long tiles = ((long long)n * a.group + tile - 1) / tile;
     long long incl = tiles;
 #pragma unroll
@@ -375,7 +378,7 @@ __device__ __forceinline__ bool row_tile(const AttnArgs& a, int idx, int tile, R
       rt.r0 = __shfl_sync(0xffffffffu, r0, l);
       rt.n = __shfl_sync(0xffffffffu, n, l);
       rt.f0 = (int)(idx - before - __shfl_sync(0xffffffffu, incl - tiles, l)) * tile;
-      rt.ctx = paged_len(a.kv, a.lens, rt.s) - rt.n;
+      rt.ctx = __shfl_sync(0xffffffffu, len, l) - rt.n;
       return true;
     }
     before += __shfl_sync(0xffffffffu, incl, 31);

@@ -127,7 +127,7 @@ template <int HD> struct TcPrefill {
 };
 
 struct TcBars {
-  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], v_raw, s_full[2], p_full[2][2], done;
+  uint64_t q_full, k_full[2], v_full[2], v_raw[2], k0_freed, freed[2], s_full[2], p_full[2][2], done;
   uint32_t tmem;
 };
 
@@ -141,6 +141,10 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
   TcBars& bar = *reinterpret_cast<TcBars*>(smem + 6 * C::TILE);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  if (threadIdx.x == 0 && box) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_k)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&map_v)) : "memory");
+  }
   // blockIdx.x = ((row tile from the last, kv head), split): the longest rows start first
   const int split = blockIdx.x % splits, unit = blockIdx.x / splits, kvh = unit % a.n_kv;
   const int units = gridDim.x / splits;
@@ -166,13 +170,14 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
     for (int i = 0; i < 2; ++i) {
       mbar_init(&bar.k_full[i], 3);  // the three gather warps
       mbar_init(&bar.v_full[i], 3);
-      mbar_init(&bar.k_empty[i], 1);
-      mbar_init(&bar.v_empty[i], 1);
+      mbar_init(&bar.v_raw[i], 1);
       mbar_init(&bar.s_full[i], 1);
       mbar_init(&bar.p_full[i][0], 4);  // the tile's four warps
       mbar_init(&bar.p_full[i][1], 4);
     }
-    mbar_init(&bar.v_raw, 1);
+    mbar_init(&bar.k0_freed, 1);
+    mbar_init(&bar.freed[0], 1);
+    mbar_init(&bar.freed[1], 1);
     mbar_init(&bar.done, 1);
     fence_mbar_init();
   }
@@ -224,6 +229,7 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
         }
         __syncwarp();
       };
+      // freed[j & 1], phase j / 2: V tile j and K tile j + 1 have been read (k0_freed: K tile 0)
       auto release = [&](uint64_t* b) {
         if (elect_one()) mma_commit(b);
         __syncwarp();
@@ -236,7 +242,7 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
       if (n > 0) wait(&bar.k_full[0], 0);
       if (ok && na > 0) qk(0, 0);
       if (ok && nb > 0) qk(1, 0);
-      if (ok && n > 0) release(&bar.k_empty[0]);
+      if (ok && n > 0) release(&bar.k0_freed);
       for (int j = 0; j < n && ok; ++j) {
         wait(&bar.v_full[j & 1], j >> 1);
 #pragma unroll
@@ -249,12 +255,11 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
             if (ok) pv(w, j, h);
           }
           if (j + 1 >= m) continue;
-          wait(&bar.k_full[(j + 1) & 1], (j + 1) >> 1);
+          if (w == 0 || j + 1 >= na) wait(&bar.k_full[(j + 1) & 1], (j + 1) >> 1);
           if (ok) qk(w, j + 1);  // in order behind the product that reads P from the same columns
         }
         if (!ok) break;
-        release(&bar.v_empty[j & 1]);
-        if (j + 1 < n) release(&bar.k_empty[(j + 1) & 1]);
+        release(&bar.freed[j & 1]);
       }
       release(&bar.done);
       warp_wait(&bar.done, 0);
@@ -299,11 +304,11 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
         if (lane == 0) mbar_arrive(full);
       };
       bool ok = true;
-      int edges = 0;
+      unsigned edges = 0;  // phase of v_raw[i] in bit i
       for (int j = 0; j < n && ok; ++j) {
         const int t0 = tile_pos(j), i = j & 1;
         const uint32_t dk = sk + i * C::TILE, dv = sv + i * C::TILE;
-        if (j >= 2) ok = warp_wait(&bar.k_empty[i], ((j >> 1) - 1) & 1);
+        if (j == 2) ok = warp_wait(&bar.k0_freed, 0);  // (K tile j - 2 of a later one: V tile j - 1 waited for it)
         if (!ok) break;
         if (!box) {
           rows(a.kv.k, dk, t0);
@@ -312,7 +317,7 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
         } else if (lane == 0) {
           mbar_arrive(&bar.k_full[i]);
         }
-        if (j >= 2) ok = warp_wait(&bar.v_empty[i], ((j >> 1) - 1) & 1);
+        if (j >= 2) ok = warp_wait(&bar.freed[i], ((j >> 1) - 1) & 1);
         if (!ok) break;
         if (!box) {
           rows(a.kv.v, dv, t0);
@@ -322,15 +327,20 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
           landed(&bar.v_full[i]);
         } else if (t0 + TN > p1 + 1 || (t0 < w0 && t0 + TN > a.sinks)) {
           // an edge tile: zeros in place of the V rows that no query row sees
-          if (warp == 9) boxes(&map_v, dv, t0, &bar.v_raw);
-          ok = warp_wait(&bar.v_raw, edges++ & 1);
-          for (int r = sub; r < TN; r += 3 * RPW) {
-            const int pos = t0 + r;
-            if (pos > p1 || (pos < w0 && pos >= a.sinks))
-              *reinterpret_cast<uint4*>(smem + 4 * C::TILE + i * C::TILE + (pc >> 3) * C::ATOM + r * 128 + ((pc & 7) << 4)) =
-                  make_uint4(0, 0, 0, 0);
+          if (warp == 9) {
+            if (lane == 0) mbar_arrive(&bar.v_full[i]);
+            boxes(&map_v, dv, t0, &bar.v_raw[i]);
+          } else {
+            ok = warp_wait(&bar.v_raw[i], edges >> i & 1);
+            edges ^= 1u << i;
+            for (int r = sub - RPW; r < TN; r += 2 * RPW) {
+              const int pos = t0 + r;
+              if (pos > p1 || (pos < w0 && pos >= a.sinks))
+                *reinterpret_cast<uint4*>(smem + (4 + i) * C::TILE + (pc >> 3) * C::ATOM + r * 128 + ((pc & 7) << 4)) =
+                    make_uint4(0, 0, 0, 0);
+            }
+            landed(&bar.v_full[i]);
           }
-          landed(&bar.v_full[i]);
         } else if (warp == 9) {
           boxes(&map_v, dv, t0, &bar.v_full[i]);
         } else if (lane == 0) {
@@ -344,14 +354,17 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
     // ---------------- softmax: one row per thread ----------------
     const int w = warp >> 2, r = threadIdx.x & 127, f = rt.f0 + w * TQ + r;
     const bool row = f < nflat;
-    const int head = kvh * a.group + (row ? f % a.group : 0);
-    const long long tok = rt.r0 + (row ? f / a.group : 0);
-    {  // this row of Q into the swizzled tile
-      const uint4* q = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + tok * a.q_row + head * a.q_head);
-      unsigned char* d = smem + w * C::TILE + r * 128;
-#pragma unroll
-      for (int c = 0; c < HD / 8; ++c)
-        *reinterpret_cast<uint4*>(d + (c >> 3) * C::ATOM + (((c & 7) ^ (r & 7)) << 4)) = row ? __ldg(q + c) : make_uint4(0, 0, 0, 0);
+    {  // this warp's 32 rows of Q into the swizzled tile, whole rows at a time
+      constexpr int PIECES = HD / 8, RPW = 32 / PIECES;
+      const int pc = lane % PIECES;
+#pragma unroll 4
+      for (int i = lane / PIECES; i < 32; i += RPW) {
+        const int x = (warp & 3) * 32 + i, fx = rt.f0 + w * TQ + x, t = min(fx, nflat - 1) / a.group;
+        const T* q = static_cast<const T*>(a.q) + (rt.r0 + t) * a.q_row + (long long)(kvh * a.group + min(fx, nflat - 1) - t * a.group) * a.q_head;
+        cpa16(sq + w * C::TILE + (pc >> 3) * C::ATOM + x * 128 + (((pc & 7) ^ (x & 7)) << 4), q + pc * 8, fx < nflat);
+      }
+      cpa_commit();
+      cpa_wait<0>();
       fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar.q_full);
@@ -446,7 +459,9 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
       tc_fence_after();
       float* part = a.part + (long long)blockIdx.x * C::SLOT;
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      T* out = static_cast<T*>(a.out) + tok * a.o_row + head * a.o_head;
+      // 16-bit rows go out through this warp's part of the Q tile (its products are
+      // done), so that stores cover whole rows
+      const uint32_t stage = sq + w * C::TILE + (warp & 3) * 32 * HD * 2;
 #pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
         uint32_t o[32];
@@ -457,23 +472,38 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
 #pragma unroll
           for (int i = 0; i < 32; ++i) o[i] = 0u;
         }
-        if (!row) continue;
         if (splits == 1) {
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
-            uint4 x;
-            x.x = pack2<T>(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
-            x.y = pack2<T>(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
-            x.z = pack2<T>(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
-            x.w = pack2<T>(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
-            *reinterpret_cast<uint4*>(out + c + i) = x;
+            uint32_t x[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              x[k] = pack2<T>(__uint_as_float(o[i + 2 * k]) * inv, __uint_as_float(o[i + 2 * k + 1]) * inv);
+            const int pc = (c + i) / 8;
+            asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(stage + lane * HD * 2 + ((pc ^ (lane & 7)) << 4)),
+                         "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
           }
-        } else {
+        } else if (row) {
           float* d = part + 4 * TQ + (long long)(w * TQ + r) * HD + c;
 #pragma unroll
           for (int i = 0; i < 32; i += 4)
             *reinterpret_cast<float4*>(d + i) = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]),
                                                             __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+        }
+      }
+      if (splits == 1) {
+        __syncwarp();
+        constexpr int PIECES = HD / 8, RPW = 32 / PIECES;
+        const int pc = lane % PIECES;
+#pragma unroll 4
+        for (int i = lane / PIECES; i < 32; i += RPW) {
+          const int fx = rt.f0 + w * TQ + (warp & 3) * 32 + i, t = fx / a.group;
+          if (fx >= nflat) break;
+          uint4 x;
+          asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+                       : "r"(stage + i * HD * 2 + ((pc ^ (i & 7)) << 4)) : "memory");
+          T* out = static_cast<T*>(a.out) + (rt.r0 + t) * a.o_row + (long long)(kvh * a.group + fx - t * a.group) * a.o_head;
+          *reinterpret_cast<uint4*>(out + pc * 8) = x;
         }
       }
       if (splits > 1 && row) {
