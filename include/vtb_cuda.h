@@ -194,7 +194,8 @@ typedef struct VtbCudaPagedKv {
 } VtbCudaPagedKv;
 
 /* New rows for the cache (f32 or the cache's type): value d of head h of row r
- * is x[r * x_row_stride + h * x_head_stride + d].  With `rope` ([n_rope][head_dim]
+ * is x[r * x_row_stride + h * x_head_stride + d] (strides of whole 16 bytes, at
+ * least head_dim).  With `rope` ([n_rope][head_dim]
  * f32, (cos, sin) of pair i of position p at [p][2i], [p][2i + 1]) keys and
  * queries are rotated by interleaved pairs (math.zig:88-104) at the row's
  * position before they are rounded to the cache's type. */
@@ -215,14 +216,14 @@ typedef struct VtbCudaPagedRows {
 int vtb_cuda_paged_append(const VtbCudaPagedKv *kv, const VtbCudaPagedRows *rows, void *stream);
 
 /* Attention over the pages.  q and out are of the cache's type; n_heads is a
- * multiple of n_kv_heads (query head h reads kv head h / (n_heads / n_kv_heads)).
+ * multiple of n_kv_heads, 128 times it at most (query head h reads kv head h / (n_heads / n_kv_heads)).
  * lens[s] counts the cached positions of sequence s, the new ones included.  A
  * query at position p sees t <= p, with window > 0 only t > p - window or
  * t < sinks.  Softmax and sums are in f32.  A query that sees nothing gets zeros. */
 typedef struct VtbCudaPagedAttn {
   const void *q;
   void *out;
-  int64_t q_row_stride, q_head_stride, out_row_stride, out_head_stride; /* elements, whole 16 bytes */
+  int64_t q_row_stride, q_head_stride, out_row_stride, out_head_stride; /* elements, whole 16 bytes, >= head_dim */
   int32_t n_heads, window, sinks;
   float scale;
   const int32_t *lens; /* device [n_seqs] */

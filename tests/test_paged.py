@@ -60,7 +60,7 @@ def test_bad_cache_is_refused(lib, buf, bad, status):
 
 
 @pytest.mark.parametrize("bad", [dict(q=None), dict(out=None), dict(q_row_stride=5), dict(out_head_stride=32), dict(n_heads=7),
-                                 dict(n_heads=0), dict(window=-1), dict(sinks=-1), dict(sinks=4), dict(lens=None),
+                                 dict(n_heads=0), dict(n_heads=258), dict(q_row_stride=0), dict(out_row_stride=32), dict(window=-1), dict(sinks=-1), dict(sinks=4), dict(lens=None),
                                  dict(scale=float("nan")), dict(scale=float("inf"))])
 def test_bad_attention_arguments_are_refused(lib, buf, bad):
     p = buf[1]
@@ -95,7 +95,7 @@ def test_bad_prefill_rows_are_refused(lib, buf):
 
 
 @pytest.mark.parametrize("bad,status", [(dict(type=1), -8), (dict(type=8), -8), (dict(n_rows=-1), -1), (dict(k=None), -1),
-                                        (dict(v=None), -1), (dict(k_row_stride=3), -1), (dict(v_head_stride=32), -1),
+                                        (dict(v=None), -1), (dict(k_row_stride=3), -1), (dict(v_head_stride=32), -1), (dict(q_row_stride=0), -1),
                                         (dict(q_out=None), -1), (dict(q=None), -1), (dict(n_heads=0), -1), (dict(seq=None), -1),
                                         (dict(pos=None), -1), (dict(n_rope=0), -1)])
 def test_bad_rows_are_refused(lib, buf, bad, status):

@@ -31,11 +31,11 @@ static int paged_view(const VtbCudaPagedKv* kv, bool need_table, PagedView* out)
   return VTB_CUDA_OK;
 }
 
-static int paged_rows_ok(const void* p, int64_t row, int64_t head, int es, int64_t hd) {
+static int paged_rows_ok(const void* p, int64_t n, int64_t row, int64_t head, int es, int64_t hd) {
   if (!p) return set_err(VTB_CUDA_ERR_INVALID_ARG, "null rows");
-  if (!aligned16(p) || !mul16(row, es) || !mul16(head, es) || row < 0 || head < hd || row > (int64_t(1) << 40) ||
+  if (!aligned16(p) || !mul16(row, es) || !mul16(head, es) || row < (n > 1 ? hd : 0) || head < hd || row > (int64_t(1) << 40) ||
       head > (int64_t(1) << 40))
-    return set_err(VTB_CUDA_ERR_INVALID_ARG, "rows must be 16-byte aligned, with strides of whole 16 bytes");
+    return set_err(VTB_CUDA_ERR_INVALID_ARG, "rows must be 16-byte aligned, with strides of whole 16 bytes and at least head_dim");
   return VTB_CUDA_OK;
 }
 
@@ -46,15 +46,15 @@ static size_t paged_workspace(int type, int group, int head_dim) {
   return d > p ? d : p;
 }
 
-static int paged_attn_args(const VtbCudaPagedKv* kv, const VtbCudaPagedAttn* p, AttnArgs* a) {
+static int paged_attn_args(const VtbCudaPagedKv* kv, const VtbCudaPagedAttn* p, int64_t rows, AttnArgs* a) {
   if (!p) return set_err(VTB_CUDA_ERR_INVALID_ARG, "null attention arguments");
   int rc = paged_view(kv, true, &a->kv);
   if (rc) return rc;
   const int es = paged_elem_bytes(kv->type);
-  if ((rc = paged_rows_ok(p->q, p->q_row_stride, p->q_head_stride, es, kv->head_dim))) return rc;
-  if ((rc = paged_rows_ok(p->out, p->out_row_stride, p->out_head_stride, es, kv->head_dim))) return rc;
-  if (p->n_heads < 1 || p->n_heads % kv->n_kv_heads || p->n_heads / kv->n_kv_heads > 4096)
-    return set_err(VTB_CUDA_ERR_INVALID_ARG, "n_heads must be a multiple of n_kv_heads");
+  if ((rc = paged_rows_ok(p->q, rows, p->q_row_stride, p->q_head_stride, es, kv->head_dim))) return rc;
+  if ((rc = paged_rows_ok(p->out, rows, p->out_row_stride, p->out_head_stride, es, kv->head_dim))) return rc;
+  if (p->n_heads < 1 || p->n_heads % kv->n_kv_heads || p->n_heads / kv->n_kv_heads > 128)
+    return set_err(VTB_CUDA_ERR_INVALID_ARG, "n_heads must be a multiple of n_kv_heads, at most 128 times it");
   if (!p->lens) return set_err(VTB_CUDA_ERR_INVALID_ARG, "null lens");
   if (!(p->scale > -INFINITY && p->scale < INFINITY)) return set_err(VTB_CUDA_ERR_INVALID_ARG, "scale must be finite");
   if (p->window < 0 || p->sinks < 0 || (p->sinks && !p->window))
@@ -72,6 +72,7 @@ static int paged_attn_args(const VtbCudaPagedKv* kv, const VtbCudaPagedAttn* p, 
   a->group = p->n_heads / kv->n_kv_heads;
   a->window = p->window;
   a->sinks = p->sinks;
+  a->tile = a->recip = 0;
   a->negate = false;
   a->scale2 = (float)((double)p->scale * 1.4426950408889634);
   if (!p->workspace || !aligned16(p->workspace) || p->workspace_bytes < paged_workspace(kv->type, a->group, kv->head_dim))
@@ -90,7 +91,7 @@ size_t vtb_cuda_paged_attn_workspace_bytes(int type, int32_t n_heads, int32_t n_
 int vtb_cuda_paged_attn_decode(const VtbCudaPagedKv* kv, const VtbCudaPagedAttn* p, void* stream) {
   cudaGetLastError();  // drop a stale error left by an unrelated earlier call
   AttnArgs a;
-  int rc = paged_attn_args(kv, p, &a);
+  int rc = paged_attn_args(kv, p, kv ? kv->n_seqs : 0, &a);
   if (rc) return rc;
   return cuda_status(launch_paged_decode(kv->type, kv->head_dim, a, (cudaStream_t)stream));
 }
@@ -99,7 +100,7 @@ int vtb_cuda_paged_attn_prefill(const VtbCudaPagedKv* kv, const VtbCudaPagedAttn
                                 void* stream) {
   cudaGetLastError();
   AttnArgs a;
-  int rc = paged_attn_args(kv, p, &a);
+  int rc = paged_attn_args(kv, p, n_rows, &a);
   if (rc) return rc;
   if (!starts || n_rows < 0 || n_rows * a.group > INT_MAX || kv->n_kv_heads > 65535)
     return set_err(VTB_CUDA_ERR_INVALID_ARG, "bad starts or n_rows");
@@ -122,10 +123,10 @@ int vtb_cuda_paged_append(const VtbCudaPagedKv* kv, const VtbCudaPagedRows* r, v
   if (r->n_rows < 0 || r->n_rows > INT_MAX) return set_err(VTB_CUDA_ERR_INVALID_ARG, "bad n_rows");
   if (r->n_rows == 0) return VTB_CUDA_OK;
   const int es = paged_elem_bytes(r->type);
-  if ((rc = paged_rows_ok(r->k, r->k_row_stride, r->k_head_stride, es, kv->head_dim))) return rc;
-  if ((rc = paged_rows_ok(r->v, r->v_row_stride, r->v_head_stride, es, kv->head_dim))) return rc;
+  if ((rc = paged_rows_ok(r->k, r->n_rows, r->k_row_stride, r->k_head_stride, es, kv->head_dim))) return rc;
+  if ((rc = paged_rows_ok(r->v, r->n_rows, r->v_row_stride, r->v_head_stride, es, kv->head_dim))) return rc;
   if (r->q) {
-    if ((rc = paged_rows_ok(r->q, r->q_row_stride, r->q_head_stride, es, kv->head_dim))) return rc;
+    if ((rc = paged_rows_ok(r->q, r->n_rows, r->q_row_stride, r->q_head_stride, es, kv->head_dim))) return rc;
     if (r->n_heads < 1 || r->n_heads > 65536 || !r->q_out || !aligned16(r->q_out))
       return set_err(VTB_CUDA_ERR_INVALID_ARG, "q needs n_heads and a 16-byte aligned q_out");
   } else if (r->q_out) {

@@ -19,8 +19,12 @@ struct AttnArgs {
   const int32_t* starts;  // prefill: first row of each sequence, then the number of rows
   int rows, n_kv, group, window, sinks;
   float scale2;  // scale * log2(e): scores are kept in units of log2
+  int tile;      // tensor-core prefill: query rows of a tile, and 2^16 / group + 1
+  int recip;
   bool negate;   // tensor-core prefill: the scale is negative (scale2 holds its size)
   float* part;   // partial results of splits
+  // Token of row x < 256 of a tile: x / group for group <= 128 (x * (recip * group - 2^16) < 2^16).
+  __device__ __forceinline__ int token(int x) const { return x * recip >> 16; }
 };
 
 // A run of cached positions as one index range: `ns` sinks, then [w0, end).
