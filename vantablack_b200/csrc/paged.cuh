@@ -143,6 +143,7 @@ template <typename T, int HD, int NT, bool F32 = Elem<T>::f32> struct Step;
 // P enters the second product as a sum of two 16-bit values, which keeps it
 // exact to 2^-17 (bf16): the output then carries its own rounding only.
 template <typename T, int HD, int NT> struct Step<T, HD, NT, false> {
+  static constexpr bool F = false;
   static constexpr int PIECES = HD / 8, KROW = HD * 2, VROW = HD * 2;  // bytes per staged row
   static constexpr int QREGS = HD / 8;
   uint32_t q[NT][QREGS];
@@ -214,6 +215,7 @@ template <typename T, int HD, int NT> struct Step<T, HD, NT, false> {
 // (jj, cc) dimensions 4 (g + 8 jj) + 2 cc + {0, 1} of lane g.  Row pitches of
 // 64 (K) and 16 bytes (V) over a multiple of 128 keep these reads conflict-free.
 template <int HD, int NT> struct Step<float, HD, NT, true> {
+  static constexpr bool F = true;
   static constexpr int PIECES = HD / 4, KROW = HD * 4 + 64, VROW = HD * 4 + 16;
   static constexpr int QREGS = HD / 4;
   float q[NT][QREGS];

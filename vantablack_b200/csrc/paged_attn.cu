@@ -44,47 +44,55 @@ __device__ __forceinline__ Span span_of(int p0, int p1, int window, int sinks) {
 
 // ======================= decode =======================
 // HBM bound: K and V are read once.  The visible positions of every (sequence,
-// kv head) are cut into tiles of 64, all tiles put in one line, and the line
+// kv head) are cut into tiles of 16 per warp, all tiles put in one line, and the line
 // cut into equal parts, one per resident CTA: a ragged batch and a single long
 // sequence load the GPU the same way, with no host knowledge of the lengths
 // (a captured call stays right as they grow).  A part that covers a whole
 // (sequence, kv head) writes its output; the others leave (max, sum, o) behind
 // and decode_join_kernel adds them in line order, so results do not depend on
-// timing.  Each of the CTA's four warps streams its own 16 positions of a tile
+// timing.  Each of the CTA's warps streams its own 16 positions of a tile
 // through a private cp.async ring, with no barrier but at a part's end.
-constexpr int DT = 64, DWARPS = 4;
+#ifndef VW32
+#define VW32 6
+#define VS32 2
+#define VW64 8
+#endif
 
 template <typename T, int HD, int NT> struct DecodeCfg {
   using S = Step<T, HD, NT>;
+  static constexpr int WARPS = S::F ? (HD == 128 ? VW32 : 8) : HD == 64 ? VW64 : 4, TILE = 16 * WARPS;
   static constexpr int STAGE = 16 * (S::KROW + S::VROW);  // bytes: one warp's K and V rows
-  static constexpr int STAGES = 3;
-  static constexpr int RED = DWARPS * 8 * (HD + 4) * 4;
-  static constexpr int SMEM = DWARPS * STAGES * STAGE + RED + DWARPS * 8 * 2 * 4;
+  static constexpr int STAGES = S::F ? (HD == 128 ? VS32 : 2) : 3;
+  static constexpr int RED = WARPS * 4 * (HD + 4) * 4;  // the warps' o of 4 query vectors
+  static constexpr int SMEM = WARPS * STAGES * STAGE + RED + WARPS * 8 * 2 * 4;
   static constexpr int SLOT = NT * 8 * (HD + 2);  // floats of one partial result
 };
 
-struct Line {  // the line of all tiles, and this CTA's place in it
-  long long total;
-  int parts;
+struct Line {  // the line of all tiles, cut into `parts`: the first `rest` of them one tile longer than `each`
+  long long total, each;
+  int parts, rest;
+  __device__ __forceinline__ long long start(int c) const { return c * each + min(c, rest); }
 };
-__device__ __forceinline__ int seq_tiles(const AttnArgs& a, int s) {
+template <int TILE> __device__ __forceinline__ int seq_tiles(const AttnArgs& a, int s) {
   const int len = paged_len(a.kv, a.lens, s);
-  return (span_of(len - 1, len - 1, a.window, a.sinks).n + DT - 1) / DT;
+  return (span_of(len - 1, len - 1, a.window, a.sinks).n + TILE - 1) / TILE;
 }
-__device__ __forceinline__ Line line_of(const AttnArgs& a, int units, int grid) {
+template <int TILE> __device__ __forceinline__ Line line_of(const AttnArgs& a, int units, int grid) {
   long long n = 0;
-  for (int s = threadIdx.x & 31; s < a.kv.n_seqs; s += 32) n += seq_tiles(a, s);
+  for (int s = threadIdx.x & 31; s < a.kv.n_seqs; s += 32) n += seq_tiles<TILE>(a, s);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
   n *= units;
-  return Line{n, (int)(n < grid ? n : grid)};
+  if (n <= grid) return Line{n, 1, (int)n, 0};
+  const long long each = n < (1ll << 32) ? (unsigned)n / (unsigned)grid : n / grid;
+  return Line{n, each, grid, (int)(n - each * grid)};
 }
 // The sequence that holds place `w` of the line, and the tiles before it.
-__device__ __forceinline__ int line_seq(const AttnArgs& a, int units, long long w, long long& before) {
+template <int TILE> __device__ __forceinline__ int line_seq(const AttnArgs& a, int units, long long w, long long& before) {
   before = 0;
   const int lane = threadIdx.x & 31;
   for (int s0 = 0; s0 < a.kv.n_seqs; s0 += 32) {
-    long long n = s0 + lane < a.kv.n_seqs ? (long long)seq_tiles(a, s0 + lane) * units : 0, incl = n;
+    long long n = s0 + lane < a.kv.n_seqs ? (long long)seq_tiles<TILE>(a, s0 + lane) * units : 0, incl = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const long long x = __shfl_up_sync(0xffffffffu, incl, o);
@@ -101,13 +109,17 @@ __device__ __forceinline__ int line_seq(const AttnArgs& a, int units, long long 
   return -1;
 }
 
-struct LineCursor {  // one tile of the line
+template <int TILE> struct LineCursor {  // one tile of the line
   int s, u, t, nt;
   Span sp;
   __device__ __forceinline__ void enter(const AttnArgs& a) {
     const int len = paged_len(a.kv, a.lens, s);
     sp = span_of(len - 1, len - 1, a.window, a.sinks);
-    nt = (sp.n + DT - 1) / DT;
+    nt = (sp.n + TILE - 1) / TILE;
+  }
+  __device__ __forceinline__ void place(long long at) {  // `at` tiles into the sequence
+    u = at < (1ll << 32) ? (int)((unsigned)at / (unsigned)nt) : (int)(at / nt);
+    t = (int)(at - (long long)u * nt);
   }
   __device__ __forceinline__ void next(const AttnArgs& a, int units) {
     if (++t < nt) return;
@@ -120,32 +132,31 @@ struct LineCursor {  // one tile of the line
 };
 
 template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(DWARPS * 32, Elem<T>::f32 ? 1 : 2)
+__global__ void __launch_bounds__(DecodeCfg<T, HD, NT>::WARPS * 32, Elem<T>::f32 ? 1 : 2)
 paged_decode_kernel(const __grid_constant__ AttnArgs a, int hgroups) {
   using C = DecodeCfg<T, HD, NT>;
   using S = Step<T, HD, NT>;
   asm volatile("griddepcontrol.launch_dependents;");
   extern __shared__ __align__(128) unsigned char smem[];
-  float* red = reinterpret_cast<float*>(smem + DWARPS * C::STAGES * C::STAGE);  // [warp][8][HD + 4]
-  float2* ml = reinterpret_cast<float2*>(red + DWARPS * 8 * (HD + 4));          // [warp][8]
+  float* red = reinterpret_cast<float*>(smem + C::WARPS * C::STAGES * C::STAGE);  // [warp][4][HD + 4]
+  float2* ml = reinterpret_cast<float2*>(red + C::WARPS * 4 * (HD + 4));          // [warp][8]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const int units = a.n_kv * hgroups;
   T* out = static_cast<T*>(a.out);
   // sequences that see nothing
   for (int s = blockIdx.x; s < a.kv.n_seqs; s += gridDim.x)
-    if (seq_tiles(a, s) == 0)
-      for (int i = threadIdx.x; i < a.n_kv * a.group * HD; i += DWARPS * 32)
+    if (seq_tiles<C::TILE>(a, s) == 0)
+      for (int i = threadIdx.x; i < a.n_kv * a.group * HD; i += C::WARPS * 32)
         out[s * a.o_row + (i / HD) * a.o_head + i % HD] = from_f<T>(0.f);
-  const Line line = line_of(a, units, gridDim.x);
+  const Line line = line_of<C::TILE>(a, units, gridDim.x);
   if ((int)blockIdx.x >= line.parts) return;
-  const long long w0 = line.total * blockIdx.x / line.parts, w1 = line.total * (blockIdx.x + 1) / line.parts;
-  LineCursor cur;
+  const long long w0 = line.start(blockIdx.x), w1 = line.start(blockIdx.x + 1);
+  LineCursor<C::TILE> cur;
   long long before;
-  cur.s = line_seq(a, units, w0, before);
+  cur.s = line_seq<C::TILE>(a, units, w0, before);
   cur.enter(a);
-  cur.u = (int)((w0 - before) / cur.nt);
-  cur.t = (int)((w0 - before) % cur.nt);
-  LineCursor ld = cur;
+  cur.place(w0 - before);
+  LineCursor<C::TILE> ld = cur;
   const int n = (int)(w1 - w0);
 
   const uint32_t ring = smem_u32(smem) + warp * C::STAGES * C::STAGE;
@@ -153,7 +164,7 @@ paged_decode_kernel(const __grid_constant__ AttnArgs a, int hgroups) {
   // the table is read one tile ahead of the copies that need it.
   int row_pos = -1, row_page = 0;
   auto look = [&]() {
-    const int i = ld.t * DT + warp * 16 + (lane & 15);
+    const int i = ld.t * C::TILE + warp * 16 + (lane & 15);
     row_pos = -1;
     if (ld.s < a.kv.n_seqs && i < ld.sp.n) {
       row_pos = ld.sp.pos(i);
@@ -185,17 +196,23 @@ paged_decode_kernel(const __grid_constant__ AttnArgs a, int hgroups) {
   }
 
   S st;
+  auto queries = [&](int s, int u) {  // the query vectors of unit u
+    const T* q = static_cast<const T*>(a.q) + s * a.q_row;
+    const int h0 = (u % hgroups) * NT * 8, kvh = u / hgroups;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int h = h0 + 8 * nt + g;
+      st.load_q(nt, h < a.group ? q + (long long)(kvh * a.group + h) * a.q_head : nullptr, t);
+    }
+  };
+  queries(cur.s, cur.u);
   float m[NT][2], l[NT][2], o[NT][HD / 16][4];
   bool fresh = true, first_part = true;
   for (int i = 0; i < n; ++i) {
     if (fresh) {
       fresh = false;
-      const T* q = static_cast<const T*>(a.q) + cur.s * a.q_row;
-      const int h0 = (cur.u % hgroups) * NT * 8, kvh = cur.u / hgroups;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const int h = h0 + 8 * nt + g;
-        st.load_q(nt, h < a.group ? q + (long long)(kvh * a.group + h) * a.q_head : nullptr, t);
         m[nt][0] = m[nt][1] = -INFINITY;
         l[nt][0] = l[nt][1] = 0.f;
 #pragma unroll
@@ -210,7 +227,7 @@ paged_decode_kernel(const __grid_constant__ AttnArgs a, int hgroups) {
       if (i + C::STAGES < n) look();
     }
     cpa_commit();
-    const int base = cur.t * DT + warp * 16;
+    const int base = cur.t * C::TILE + warp * 16;
     if (base < cur.sp.n) {
       const uint32_t kb = ring + (i % C::STAGES) * C::STAGE;
       float s[NT][4];
@@ -234,7 +251,9 @@ paged_decode_kernel(const __grid_constant__ AttnArgs a, int hgroups) {
     // ---- end of this CTA's share of (sequence, unit): join the four warps ----
     fresh = true;
     const bool whole = cur.t + 1 == cur.nt && i >= cur.nt - 1;
-    const int h0 = (cur.u % hgroups) * NT * 8, kvh = cur.u / hgroups;
+    const int h0 = (cur.u % hgroups) * NT * 8, kvh = cur.u / hgroups, seq = cur.s;
+    cur.next(a, units);
+    if (i + 1 < n) queries(cur.s, cur.u);  // on their way while the warps are joined
     float* slot = a.part + (2ll * blockIdx.x + (first_part ? 0 : 1)) * C::SLOT;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -249,86 +268,117 @@ paged_decode_kernel(const __grid_constant__ AttnArgs a, int hgroups) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         float M = -INFINITY;
-        for (int w = 0; w < DWARPS; ++w) M = fmaxf(M, ml[w * 8 + 2 * t + c].x);
+        for (int w = 0; w < C::WARPS; ++w) M = fmaxf(M, ml[w * 8 + 2 * t + c].x);
         f[c] = exp2f(m[nt][c] - (M == -INFINITY ? 0.f : M));
       }
-      float* mine = red + (warp * 8 + 2 * t) * (HD + 4);
 #pragma unroll
-      for (int j = 0; j < HD / 16; ++j)
+      for (int v0 = 0; v0 < 8; v0 += 4) {  // vectors v0 ... v0 + 3 of the eight
+        const int heads = min(4, a.group - h0 - 8 * nt - v0);
+        if (heads <= 0) break;
+        if (t >> 1 == v0 >> 2) {
+          float* mine = red + (warp * 4 + 2 * (t & 1)) * (HD + 4);
 #pragma unroll
-        for (int hi = 0; hi < 2; ++hi) {
-          const int d = S::dim(j, hi, g);
-          mine[d] = o[nt][j][2 * hi] * f[0];
-          mine[HD + 4 + d] = o[nt][j][2 * hi + 1] * f[1];
+          for (int j = 0; j < HD / 16; ++j)
+#pragma unroll
+            for (int hi = 0; hi < 2; ++hi) {
+              const int d = S::dim(j, hi, g);
+              mine[d] = o[nt][j][2 * hi] * f[0];
+              mine[HD + 4 + d] = o[nt][j][2 * hi + 1] * f[1];
+            }
         }
-      __syncthreads();
-      const int heads = min(8, a.group - h0 - 8 * nt);
-      for (int x = threadIdx.x; x < heads * HD; x += DWARPS * 32) {
-        const int h = x / HD, d = x % HD;
-        float M = -INFINITY, L = 0.f, acc = 0.f;
-        for (int w = 0; w < DWARPS; ++w) M = fmaxf(M, ml[w * 8 + h].x);
-        const float b = M == -INFINITY ? 0.f : M;
-        for (int w = 0; w < DWARPS; ++w) {
-          const float2 v = ml[w * 8 + h];
-          L += v.y * exp2f(v.x - b);
-          acc += red[(w * 8 + h) * (HD + 4) + d];
-        }
-        if (whole) {
-          out[cur.s * a.o_row + (long long)(kvh * a.group + h0 + 8 * nt + h) * a.o_head + d] =
-              from_f<T>(L == 0.f ? 0.f : acc / L);
-        } else {
-          slot[NT * 16 + (8 * nt + h) * HD + d] = acc;
-          if (d == 0) {
-            slot[8 * nt + h] = M;
-            slot[NT * 8 + 8 * nt + h] = L;
+        __syncthreads();
+        for (int x = threadIdx.x; x < heads * HD; x += C::WARPS * 32) {
+          const int h = x / HD, d = x % HD;
+          float M = -INFINITY, L = 0.f, acc = 0.f;
+          for (int w = 0; w < C::WARPS; ++w) M = fmaxf(M, ml[w * 8 + v0 + h].x);
+          const float b = M == -INFINITY ? 0.f : M;
+          for (int w = 0; w < C::WARPS; ++w) {
+            const float2 v = ml[w * 8 + v0 + h];
+            L += v.y * exp2f(v.x - b);
+            acc += red[(w * 4 + h) * (HD + 4) + d];
+          }
+          const int hu = 8 * nt + v0 + h;  // head of the unit
+          if (whole) {
+            out[seq * a.o_row + (long long)(kvh * a.group + h0 + hu) * a.o_head + d] = from_f<T>(L == 0.f ? 0.f : acc / L);
+          } else {
+            slot[NT * 16 + hu * HD + d] = acc;
+            if (d == 0) {
+              slot[hu] = M;
+              slot[NT * 8 + hu] = L;
+            }
           }
         }
+        __syncthreads();  // ml and red are free again
       }
-      __syncthreads();  // ml and red are free again
     }
     first_part = false;
-    cur.next(a, units);
   }
   cpa_wait<0>();
 }
 
 // Adds the parts of each (sequence, unit) that a boundary of the line cuts: CTA
-// b looks at boundary b + 1 and works only if it is the first one in its unit.
+// (b, h) looks at boundary b + 1 and works only if it is the first one in its
+// unit, on head h of the unit.  The plan is made before the wait, while the
+// decode kernel still runs.
+constexpr int JOIN_MAX = 512;  // parts there can be (resident CTAs of a decode call)
 template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(256) paged_decode_join_kernel(const __grid_constant__ AttnArgs a, int hgroups, int grid) {
+__global__ void __launch_bounds__(HD) paged_decode_join_kernel(const __grid_constant__ AttnArgs a, int hgroups, int grid) {
   using C = DecodeCfg<T, HD, NT>;
+  __shared__ float weight[JOIN_MAX];
+  __shared__ float red[2 * HD / 32];
   const int units = a.n_kv * hgroups;
-  const Line line = line_of(a, units, grid);
-  const int c = blockIdx.x + 1;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (c >= line.parts) return;
-  const long long w = line.total * c / line.parts, prev = line.total * (c - 1) / line.parts;
-  long long before;
-  const int s = line_seq(a, units, w, before);
-  const int nt = seq_tiles(a, s);
-  const int u = (int)((w - before) / nt);
-  const long long u0 = before + (long long)u * nt, u1 = u0 + nt;
-  if (w == u0 || prev > u0) return;  // no cut here, or not the unit's first
-  int last = c;
-  while (last + 1 < line.parts && line.total * (last + 1) / line.parts < u1) ++last;
-  const float* p0 = a.part + (2ll * (c - 1) + (prev == u0 ? 0 : 1)) * C::SLOT;
-  const int h0 = (u % hgroups) * NT * 8, kvh = u / hgroups, heads = min(8 * NT, a.group - h0);
-  T* out = static_cast<T*>(a.out) + s * a.o_row + (long long)(kvh * a.group + h0) * a.o_head;
-  for (int x = threadIdx.x; x < heads * HD; x += blockDim.x) {
-    const int h = x / HD, d = x % HD;
-    float M = p0[h];
-    for (int i = c; i <= last; ++i) M = fmaxf(M, a.part[2ll * i * C::SLOT + h]);
-    const float b = M == -INFINITY ? 0.f : M;
-    float e = exp2f(p0[h] - b), L = p0[NT * 8 + h] * e, acc = p0[NT * 16 + h * HD + d] * e;
-#pragma unroll 4
-    for (int i = c; i <= last; ++i) {
-      const float* p = a.part + 2ll * i * C::SLOT;
-      e = exp2f(p[h] - b);
-      L += p[NT * 8 + h] * e;
-      acc += p[NT * 16 + h * HD + d] * e;
-    }
-    out[h * a.o_head + d] = from_f<T>(L == 0.f ? 0.f : acc / L);
+  const Line line = line_of<C::TILE>(a, units, grid);
+  const int c = blockIdx.x + 1, h = blockIdx.y, d = threadIdx.x, warp = d >> 5, lane = d & 31;
+  bool mine = c < line.parts;
+  long long before = 0, u0 = 0, w = 0;
+  LineCursor<C::TILE> cur;
+  int n = 0;  // parts of the unit
+  if (mine) {
+    w = line.start(c);
+    cur.s = line_seq<C::TILE>(a, units, w, before);
+    cur.enter(a);
+    cur.place(w - before);
+    u0 = w - cur.t;
+    mine = cur.t > 0 && line.start(c - 1) <= u0 && (cur.u % hgroups) * NT * 8 + h < a.group;
+    if (mine)
+      for (n = 1; c - 1 + n < line.parts && line.start(c - 1 + n) < u0 + cur.nt; ++n) {
+      }
   }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (!mine) return;
+  // The first part is the last of its CTA (slot 1) unless the CTA began with this unit; the others are first ones.
+  const float* first = a.part + (2ll * (c - 1) + (line.start(c - 1) == u0 ? 0 : 1)) * C::SLOT;
+  auto slot = [&](int i) { return i ? a.part + 2ll * (c - 1 + i) * C::SLOT : first; };
+  float M = -INFINITY;
+  for (int i = d; i < n; i += HD) {
+    const float m = slot(i)[h];
+    weight[i] = m;
+    M = fmaxf(M, m);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  if (lane == 0) red[warp] = M;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < HD / 32; ++i) M = fmaxf(M, red[i]);
+  const float b = M == -INFINITY ? 0.f : M;
+  float L = 0.f;
+  for (int i = d; i < n; i += HD) {
+    const float e = exp2f(weight[i] - b);
+    weight[i] = e;
+    L += slot(i)[NT * 8 + h] * e;
+  }
+  L = warp_sum(L);
+  if (lane == 0) red[HD / 32 + warp] = L;
+  __syncthreads();
+  L = 0.f;
+#pragma unroll
+  for (int i = 0; i < HD / 32; ++i) L += red[HD / 32 + i];
+  float acc = 0.f;
+#pragma unroll 8
+  for (int i = 0; i < n; ++i) acc += slot(i)[NT * 16 + h * HD + d] * weight[i];
+  static_cast<T*>(a.out)[cur.s * a.o_row + (long long)((cur.u / hgroups) * a.group + (cur.u % hgroups) * NT * 8 + h) * a.o_head + d] =
+      from_f<T>(L == 0.f ? 0.f : acc / L);
 }
 
 // ======================= prefill =======================
@@ -506,14 +556,14 @@ static cudaError_t launch_decode_t(const AttnArgs& a, int hgroups, int grid, cud
   // no more CTAs than tiles there can be
   const long long cap = (long long)a.kv.pages_per_seq << a.kv.page_shift;
   const long long vis = a.window && a.window + (long long)a.sinks < cap ? a.window + (long long)a.sinks : cap;
-  const long long most = a.kv.n_seqs * (long long)a.n_kv * hgroups * ((vis + DT - 1) / DT);
+  const long long most = a.kv.n_seqs * (long long)a.n_kv * hgroups * ((vis + C::TILE - 1) / C::TILE);
   if (most < grid) grid = (int)(most > 0 ? most : 1);
-  paged_decode_kernel<T, HD, NT><<<grid, DWARPS * 32, C::SMEM, st>>>(a, hgroups);
+  paged_decode_kernel<T, HD, NT><<<grid, C::WARPS * 32, C::SMEM, st>>>(a, hgroups);
   if ((e = cudaGetLastError())) return e;
-  if (vis <= DT || grid == 1) return cudaSuccess;  // one tile per unit: nothing is cut
+  if (vis <= C::TILE || grid == 1) return cudaSuccess;  // one tile per unit: nothing is cut
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid - 1);
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3(grid - 1, a.group < 8 * NT ? a.group : 8 * NT);
+  cfg.blockDim = dim3(HD);
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -524,7 +574,10 @@ static cudaError_t launch_decode_t(const AttnArgs& a, int hgroups, int grid, cud
 }
 
 // Resident CTAs that share a decode call's line, and the workspace they need.
-static int decode_grid(int type) { return sm_count(current_device()) * (type == F32 ? 1 : 2); }
+static int decode_grid(int type) {
+  const int n = sm_count(current_device()) * (type == F32 ? 1 : 2);
+  return n < JOIN_MAX ? n : JOIN_MAX;
+}
 size_t paged_decode_workspace(int type, int group, int head_dim) {
   const int nt = group > 8 ? 2 : 1;
   return (size_t)2 * decode_grid(type) * nt * 8 * (head_dim + 2) * sizeof(float);
