@@ -52,17 +52,12 @@ __device__ __forceinline__ Span span_of(int p0, int p1, int window, int sinks) {
 // and decode_join_kernel adds them in line order, so results do not depend on
 // timing.  Each of the CTA's warps streams its own 16 positions of a tile
 // through a private cp.async ring, with no barrier but at a part's end.
-#ifndef VW32
-#define VW32 6
-#define VS32 2
-#define VW64 8
-#endif
 
 template <typename T, int HD, int NT> struct DecodeCfg {
   using S = Step<T, HD, NT>;
-  static constexpr int WARPS = S::F ? (HD == 128 ? VW32 : 8) : HD == 64 ? VW64 : 4, TILE = 16 * WARPS;
+  static constexpr int WARPS = S::F ? (HD == 128 ? 6 : 8) : HD == 64 ? 8 : 4, TILE = 16 * WARPS;
   static constexpr int STAGE = 16 * (S::KROW + S::VROW);  // bytes: one warp's K and V rows
-  static constexpr int STAGES = S::F ? (HD == 128 ? VS32 : 2) : 3;
+  static constexpr int STAGES = S::F ? 2 : 3;
   static constexpr int RED = WARPS * 4 * (HD + 4) * 4;  // the warps' o of 4 query vectors
   static constexpr int SMEM = WARPS * STAGES * STAGE + RED + WARPS * 8 * 2 * 4;
   static constexpr int SLOT = NT * 8 * (HD + 2);  // floats of one partial result
@@ -137,6 +132,7 @@ paged_decode_kernel(const __grid_constant__ AttnArgs a, int hgroups) {
   using C = DecodeCfg<T, HD, NT>;
   using S = Step<T, HD, NT>;
   asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   extern __shared__ __align__(128) unsigned char smem[];
   float* red = reinterpret_cast<float*>(smem + C::WARPS * C::STAGES * C::STAGE);  // [warp][4][HD + 4]
   float2* ml = reinterpret_cast<float2*>(red + C::WARPS * 4 * (HD + 4));          // [warp][8]
@@ -149,7 +145,12 @@ paged_decode_kernel(const __grid_constant__ AttnArgs a, int hgroups) {
       for (int i = threadIdx.x; i < a.n_kv * a.group * HD; i += C::WARPS * 32)
         out[s * a.o_row + (i / HD) * a.o_head + i % HD] = from_f<T>(0.f);
   const Line line = line_of<C::TILE>(a, units, gridDim.x);
-  if ((int)blockIdx.x >= line.parts) return;
+  // What the join does for this CTA: n parts of unit (s, u), the first of them in this CTA's slot.
+  int4* todo = reinterpret_cast<int4*>(a.part + 2ll * gridDim.x * C::SLOT) + blockIdx.x;
+  if ((int)blockIdx.x >= line.parts) {
+    if (threadIdx.x == 0) *todo = make_int4(0, 0, 0, 0);
+    return;
+  }
   const long long w0 = line.start(blockIdx.x), w1 = line.start(blockIdx.x + 1);
   LineCursor<C::TILE> cur;
   long long before;
@@ -207,7 +208,7 @@ paged_decode_kernel(const __grid_constant__ AttnArgs a, int hgroups) {
   };
   queries(cur.s, cur.u);
   float m[NT][2], l[NT][2], o[NT][HD / 16][4];
-  bool fresh = true, first_part = true;
+  bool fresh = true, first_part = true, left = false;
   for (int i = 0; i < n; ++i) {
     if (fresh) {
       fresh = false;
@@ -252,6 +253,15 @@ paged_decode_kernel(const __grid_constant__ AttnArgs a, int hgroups) {
     fresh = true;
     const bool whole = cur.t + 1 == cur.nt && i >= cur.nt - 1;
     const int h0 = (cur.u % hgroups) * NT * 8, kvh = cur.u / hgroups, seq = cur.s;
+    if (cur.t + 1 < cur.nt && i >= cur.t) {  // begins here and goes on in the CTAs behind
+      left = true;
+      if (threadIdx.x == 0) {
+        const long long end = w0 + i - cur.t + cur.nt;
+        int parts = 1;
+        while ((int)blockIdx.x + parts < line.parts && line.start(blockIdx.x + parts) < end) ++parts;
+        *todo = make_int4(seq, cur.u, parts, first_part ? 0 : 1);
+      }
+    }
     cur.next(a, units);
     if (i + 1 < n) queries(cur.s, cur.u);  // on their way while the warps are joined
     float* slot = a.part + (2ll * blockIdx.x + (first_part ? 0 : 1)) * C::SLOT;
@@ -314,41 +324,26 @@ paged_decode_kernel(const __grid_constant__ AttnArgs a, int hgroups) {
     first_part = false;
   }
   cpa_wait<0>();
+  if (threadIdx.x == 0 && !left) *todo = make_int4(0, 0, 0, 0);
 }
 
-// Adds the parts of each (sequence, unit) that a boundary of the line cuts: CTA
-// (b, h) looks at boundary b + 1 and works only if it is the first one in its
-// unit, on head h of the unit.  The plan is made before the wait, while the
-// decode kernel still runs.
+// Adds the parts of each (sequence, unit) that is cut: CTA (c, h) does what CTA c
+// of the decode kernel left to do, for head h of the unit.
 constexpr int JOIN_MAX = 512;  // parts there can be (resident CTAs of a decode call)
 template <typename T, int HD, int NT>
-__global__ void __launch_bounds__(HD) paged_decode_join_kernel(const __grid_constant__ AttnArgs a, int hgroups, int grid) {
+__global__ void __launch_bounds__(HD) paged_decode_join_kernel(const __grid_constant__ AttnArgs a, int hgroups) {
   using C = DecodeCfg<T, HD, NT>;
+  asm volatile("griddepcontrol.launch_dependents;");
   __shared__ float weight[JOIN_MAX];
   __shared__ float red[2 * HD / 32];
-  const int units = a.n_kv * hgroups;
-  const Line line = line_of<C::TILE>(a, units, grid);
-  const int c = blockIdx.x + 1, h = blockIdx.y, d = threadIdx.x, warp = d >> 5, lane = d & 31;
-  bool mine = c < line.parts;
-  long long before = 0, u0 = 0, w = 0;
-  LineCursor<C::TILE> cur;
-  int n = 0;  // parts of the unit
-  if (mine) {
-    w = line.start(c);
-    cur.s = line_seq<C::TILE>(a, units, w, before);
-    cur.enter(a);
-    cur.place(w - before);
-    u0 = w - cur.t;
-    mine = cur.t > 0 && line.start(c - 1) <= u0 && (cur.u % hgroups) * NT * 8 + h < a.group;
-    if (mine)
-      for (n = 1; c - 1 + n < line.parts && line.start(c - 1 + n) < u0 + cur.nt; ++n) {
-      }
-  }
+  const int c = blockIdx.x, h = blockIdx.y, d = threadIdx.x, warp = d >> 5, lane = d & 31;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (!mine) return;
-  // The first part is the last of its CTA (slot 1) unless the CTA began with this unit; the others are first ones.
-  const float* first = a.part + (2ll * (c - 1) + (line.start(c - 1) == u0 ? 0 : 1)) * C::SLOT;
-  auto slot = [&](int i) { return i ? a.part + 2ll * (c - 1 + i) * C::SLOT : first; };
+  const int4 job = reinterpret_cast<const int4*>(a.part + 2ll * gridDim.x * C::SLOT)[c];
+  const int n = job.z, u = job.y;  // parts of the unit (0: nothing to do)
+  if (n == 0 || (u % hgroups) * NT * 8 + h >= a.group) return;
+  // the first part lies in slot job.w of CTA c, the others are the first ones of the CTAs behind it
+  const float* first = a.part + (2ll * c + job.w) * C::SLOT;
+  auto slot = [&](int i) { return i ? a.part + 2ll * (c + i) * C::SLOT : first; };
   float M = -INFINITY;
   for (int i = d; i < n; i += HD) {
     const float m = slot(i)[h];
@@ -377,7 +372,7 @@ __global__ void __launch_bounds__(HD) paged_decode_join_kernel(const __grid_cons
   float acc = 0.f;
 #pragma unroll 8
   for (int i = 0; i < n; ++i) acc += slot(i)[NT * 16 + h * HD + d] * weight[i];
-  static_cast<T*>(a.out)[cur.s * a.o_row + (long long)((cur.u / hgroups) * a.group + (cur.u % hgroups) * NT * 8 + h) * a.o_head + d] =
+  static_cast<T*>(a.out)[job.x * a.o_row + (long long)((u / hgroups) * a.group + (u % hgroups) * NT * 8 + h) * a.o_head + d] =
       from_f<T>(L == 0.f ? 0.f : acc / L);
 }
 
@@ -547,6 +542,24 @@ __global__ void __launch_bounds__(PWARPS * 32, 1) paged_prefill_kernel(const __g
 }
 
 // ======================= launches =======================
+// Programmatic dependent launch: the kernel may start while its predecessor on
+// the stream still runs, and waits for it (griddepcontrol.wait) before it reads
+// or writes anything.
+template <typename K, typename... A>
+static cudaError_t launch_dependent(K kern, dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
 template <typename T, int HD, int NT>
 static cudaError_t launch_decode_t(const AttnArgs& a, int hgroups, int grid, cudaStream_t st) {
   using C = DecodeCfg<T, HD, NT>;
@@ -558,19 +571,10 @@ static cudaError_t launch_decode_t(const AttnArgs& a, int hgroups, int grid, cud
   const long long vis = a.window && a.window + (long long)a.sinks < cap ? a.window + (long long)a.sinks : cap;
   const long long most = a.kv.n_seqs * (long long)a.n_kv * hgroups * ((vis + C::TILE - 1) / C::TILE);
   if (most < grid) grid = (int)(most > 0 ? most : 1);
-  paged_decode_kernel<T, HD, NT><<<grid, C::WARPS * 32, C::SMEM, st>>>(a, hgroups);
-  if ((e = cudaGetLastError())) return e;
-  if (vis <= C::TILE || grid == 1) return cudaSuccess;  // one tile per unit: nothing is cut
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid - 1, a.group < 8 * NT ? a.group : 8 * NT);
-  cfg.blockDim = dim3(HD);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_decode_join_kernel<T, HD, NT>, a, hgroups, grid);
+  if ((e = launch_dependent(paged_decode_kernel<T, HD, NT>, dim3(grid), dim3(C::WARPS * 32), C::SMEM, st, a, hgroups))) return e;
+  if (vis <= C::TILE) return cudaSuccess;  // one tile per unit: nothing is cut
+  return launch_dependent(paged_decode_join_kernel<T, HD, NT>, dim3(grid, a.group < 8 * NT ? a.group : 8 * NT), dim3(HD), 0, st, a,
+                          hgroups);
 }
 
 // Resident CTAs that share a decode call's line, and the workspace they need.
@@ -580,7 +584,7 @@ static int decode_grid(int type) {
 }
 size_t paged_decode_workspace(int type, int group, int head_dim) {
   const int nt = group > 8 ? 2 : 1;
-  return (size_t)2 * decode_grid(type) * nt * 8 * (head_dim + 2) * sizeof(float);
+  return decode_grid(type) * ((size_t)2 * nt * 8 * (head_dim + 2) * sizeof(float) + sizeof(int4));
 }
 
 cudaError_t launch_paged_decode(int type, int head_dim, const AttnArgs& a, cudaStream_t st) {

@@ -663,16 +663,7 @@ static cudaError_t launch_prefill_tc_t(AttnArgs a, cudaStream_t st) {
   const unsigned grid = (unsigned)(items < sm_count(dev) ? items : sm_count(dev));
   paged_prefill_tc_kernel<T, HD><<<grid, TC_THREADS, C::SMEM, st>>>(a, map_k, map_v, map_q, (int)items, (int)splits, box);
   if ((e = cudaGetLastError()) || splits == 1) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(units * 16));
-  cfg.blockDim = dim3(256);
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_prefill_join_kernel<T, HD>, a, (int)splits);
+  return launch_dependent(paged_prefill_join_kernel<T, HD>, dim3((unsigned)(units * 16)), dim3(256), 0, st, a, (int)splits);
 }
 
 cudaError_t launch_paged_prefill_tc(int type, int head_dim, const AttnArgs& a, cudaStream_t st) {
