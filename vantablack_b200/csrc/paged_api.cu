@@ -42,7 +42,7 @@ static int paged_rows_ok(const void* p, int64_t n, int64_t row, int64_t head, in
 // One workspace serves both attention calls.
 static size_t paged_workspace(int type, int group, int head_dim) {
   const size_t d = paged_decode_workspace(type, group, head_dim);
-  const size_t p = type == F32 ? 0 : paged_prefill_tc_workspace(head_dim);
+  const size_t p = type == F32 ? paged_prefill_f32_workspace(head_dim) : paged_prefill_tc_workspace(head_dim);
   return d > p ? d : p;
 }
 

@@ -376,20 +376,7 @@ __global__ void __launch_bounds__(HD) paged_decode_join_kernel(const __grid_cons
       from_f<T>(L == 0.f ? 0.f : acc / L);
 }
 
-// ======================= prefill =======================
-// The query rows of one kv head are the pairs (token, head of the group) in
-// token order, flattened, so any group size fills the 128 rows of a CTA; the
-// CTA walks the positions that its rows see in tiles of 64 staged through two
-// cp.async stages.  Warp w owns rows 16 w .. 16 w + 15.
-constexpr int PQ = 128, PT = 64, PWARPS = 8;
-
-template <typename T, int HD> struct PrefillCfg {
-  using S = Step<T, HD, 2>;
-  static constexpr int STAGE = PT * (S::KROW + S::VROW);
-  static constexpr int OUT = PWARPS * 16 * (HD + 4) * 4;
-  static constexpr int SMEM = 2 * STAGE > OUT ? 2 * STAGE : OUT;
-};
-
+// ======================= rows of a chunk (prefill) =======================
 // Rows [r0, r0 + n) of sequence s; tile `idx` of the line of all sequences' row
 // tiles gives (s, first flattened row).  Bad starts set the error word.
 struct RowTile {
@@ -433,112 +420,6 @@ __device__ __forceinline__ bool row_tile(const AttnArgs& a, int idx, int tile, R
     before += __shfl_sync(0xffffffffu, incl, 31);
   }
   return false;
-}
-
-template <typename T, int HD>
-__global__ void __launch_bounds__(PWARPS * 32, 1) paged_prefill_kernel(const __grid_constant__ AttnArgs a) {
-  using C = PrefillCfg<T, HD>;
-  using S = Step<T, HD, 2>;
-  extern __shared__ __align__(128) unsigned char smem[];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  RowTile rt;
-  if (!row_tile(a, gridDim.x - 1 - blockIdx.x, PQ, rt)) return;
-  const int kvh = blockIdx.y, nflat = rt.n * a.group;
-  const int last = min(rt.f0 + PQ, nflat) - 1;
-  const Span sp = span_of(max(0, rt.ctx + rt.f0 / a.group), rt.ctx + last / a.group, a.window, a.sinks);
-  const int tiles = (sp.n + PT - 1) / PT;
-
-  const uint32_t sbase = smem_u32(smem);
-  auto load = [&](int tile) {
-    const uint32_t kd = sbase + (tile & 1) * C::STAGE, vd = kd + PT * S::KROW;
-    for (int x = threadIdx.x; x < PT * S::PIECES; x += PWARPS * 32) {
-      const int r = x / S::PIECES, pc = x % S::PIECES, i = tile * PT + r;
-      const bool live = i < sp.n;
-      long long src = pc * 16;
-      if (live) {
-        const int pos = sp.pos(i);
-        src += page_row(a.kv, a.kv.table[rt.s * a.kv.table_stride + (pos >> a.kv.page_shift)], pos) + kvh * a.kv.head_stride;
-      }
-      cpa16(kd + S::k_off(r, pc), a.kv.k + src, live);
-      cpa16(vd + S::v_off(r, pc), a.kv.v + src, live);
-    }
-  };
-  if (tiles > 0) load(0);
-  cpa_commit();
-
-  S st;
-  float m[2][2], l[2][2], o[2][HD / 16][4];
-  int qp[2][2];  // position of vectors 8 nt + 2t + c
-#pragma unroll
-  for (int nt = 0; nt < 2; ++nt) {
-    const int f = rt.f0 + warp * 16 + nt * 8;
-    const T* q = nullptr;
-    if (f + g < nflat)
-      q = static_cast<const T*>(a.q) + (rt.r0 + (f + g) / a.group) * a.q_row +
-          (long long)(kvh * a.group + (f + g) % a.group) * a.q_head;
-    st.load_q(nt, q, t);
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const int fv = f + 2 * t + c;
-      qp[nt][c] = fv < nflat ? rt.ctx + fv / a.group : -1;
-      m[nt][c] = -INFINITY;
-      l[nt][c] = 0.f;
-    }
-#pragma unroll
-    for (int j = 0; j < HD / 16; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
-  }
-  for (int tile = 0; tile < tiles; ++tile) {
-    if (tile + 1 < tiles) load(tile + 1);
-    cpa_commit();
-    cpa_wait<1>();
-    __syncthreads();
-    const uint32_t kb = sbase + (tile & 1) * C::STAGE, vb = kb + PT * S::KROW;
-#pragma unroll 1
-    for (int r = 0; r < PT && tile * PT + r < sp.n; r += 16) {
-      float s[2][4];
-      st.scores(kb + S::k_off(r, 0), lane, s);
-#pragma unroll
-      for (int hi = 0; hi < 2; ++hi) {
-        const int i = tile * PT + r + g + 8 * hi, pos = i < sp.n ? sp.pos(i) : 0x7fffffff;
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const bool see = pos <= qp[nt][c] && (!a.window || pos > qp[nt][c] - a.window || pos < a.sinks);
-            s[nt][2 * hi + c] = see ? s[nt][2 * hi + c] * a.scale2 : -INFINITY;
-          }
-      }
-      float f[2][2];
-      const bool moved = softmax_step<2>(s, m, l, f);
-      st.pv(vb + S::v_off(r, 0), lane, s, f, moved, o);
-    }
-    __syncthreads();
-  }
-  // ---- output through shared memory, whole rows ----
-  cpa_wait<0>();
-  __syncthreads();
-  float* mine = reinterpret_cast<float*>(smem) + warp * 16 * (HD + 4);
-#pragma unroll
-  for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-#pragma unroll
-      for (int off = 4; off < 32; off <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], off);
-      const float inv = l[nt][c] == 0.f ? 0.f : 1.f / l[nt][c];
-#pragma unroll
-      for (int j = 0; j < HD / 16; ++j)
-#pragma unroll
-        for (int hi = 0; hi < 2; ++hi)
-          mine[(8 * nt + 2 * t + c) * (HD + 4) + S::dim(j, hi, g)] = o[nt][j][2 * hi + c] * inv;
-    }
-  __syncwarp();
-  T* out = static_cast<T*>(a.out);
-  for (int r = 0; r < 16; ++r) {
-    const int f = rt.f0 + warp * 16 + r;
-    if (f >= nflat) break;
-    T* row = out + (rt.r0 + f / a.group) * a.o_row + (long long)(kvh * a.group + f % a.group) * a.o_head;
-    for (int d = lane; d < HD; d += 32) row[d] = from_f<T>(mine[r * (HD + 4) + d]);
-  }
 }
 
 // ======================= launches =======================
@@ -602,21 +483,6 @@ cudaError_t launch_paged_decode(int type, int head_dim, const AttnArgs& a, cudaS
   if (head_dim == 64) VTB_DEC(__nv_bfloat16, 64);
   VTB_DEC(__nv_bfloat16, 128);
 #undef VTB_DEC
-}
-
-template <typename T, int HD>
-static cudaError_t launch_prefill_t(const AttnArgs& a, cudaStream_t st) {
-  using C = PrefillCfg<T, HD>;
-  cudaError_t e = ensure_smem_attr<paged_prefill_kernel<T, HD>>(current_device(), C::SMEM);
-  if (e) return e;
-  // row tiles: at most one ragged tile per sequence more than full ones
-  const long long tiles = (long long)a.rows * a.group / PQ + a.kv.n_seqs;
-  paged_prefill_kernel<T, HD><<<dim3((unsigned)tiles, a.n_kv), PWARPS * 32, C::SMEM, st>>>(a);
-  return cudaGetLastError();
-}
-
-cudaError_t launch_paged_prefill_f32(int head_dim, const AttnArgs& a, cudaStream_t st) {
-  return head_dim == 64 ? launch_prefill_t<float, 64>(a, st) : launch_prefill_t<float, 128>(a, st);
 }
 
 }  // namespace vtb

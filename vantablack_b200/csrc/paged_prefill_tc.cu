@@ -84,6 +84,11 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* v) {
       "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
       ::VTB_I8(v, 0), VTB_I8(v, 8), VTB_I8(v, 16), VTB_I8(v, 24), "r"(addr) : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+      ::VTB_I8(v, 0), VTB_I8(v, 8), "r"(addr) : "memory");
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ float ex2(float x) {
@@ -554,37 +559,38 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
   }
 }
 
-// Adds the splits of 256 rows, 16 rows per CTA: out = sum_i o_i 2^(m_i - M) / sum_i l_i 2^(m_i - M).
-template <typename T, int HD>
+// Adds the splits of an item's TILES x 128 rows, 16 rows per CTA:
+// out = sum_i o_i 2^(m_i - M) / sum_i l_i 2^(m_i - M).
+template <typename T, int HD, int TILES>
 __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const __grid_constant__ AttnArgs a, int splits) {
-  using C = TcPrefill<HD>;
-  const int unit = blockIdx.x >> 4, kvh = unit % a.n_kv, units = gridDim.x >> 4;
+  constexpr int ROWS = TILES * TQ, SLOT = ROWS * (HD + 2), CTAS = ROWS / 16, V = 16 / sizeof(T), LANES = HD / V;
+  const int unit = blockIdx.x / CTAS, kvh = unit % a.n_kv, units = gridDim.x / CTAS;
   RowTile rt;
-  const bool any = row_tile(a, units / a.n_kv - 1 - unit / a.n_kv, 2 * a.tile, rt);
+  const bool any = row_tile(a, units / a.n_kv - 1 - unit / a.n_kv, TILES * a.tile, rt);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   if (!any) return;
-  constexpr int LANES = HD / 8;  // threads per row, 8 values each
   for (int x = threadIdx.x; x < 16 * LANES; x += 256) {
-    const int r = (blockIdx.x & 15) * 16 + x / LANES, c = (x % LANES) * 8;  // row r % TQ of tile r / TQ
+    const int r = (blockIdx.x % CTAS) * 16 + x / LANES, c = (x % LANES) * V;  // row r % TQ of tile r / TQ
     const int f = rt.f0 + (r / TQ) * a.tile + r % TQ;
     if (r % TQ >= a.tile || f >= rt.n * a.group) continue;
-    const float* p = a.part + (long long)unit * splits * C::SLOT;
-    float M = -INFINITY, L = 0.f, acc[8] = {};
-    for (int i = 0; i < splits; ++i) M = fmaxf(M, p[(long long)i * C::SLOT + r]);
+    const float* p = a.part + (long long)unit * splits * SLOT;
+    float M = -INFINITY, L = 0.f, acc[V] = {};
+    for (int i = 0; i < splits; ++i) M = fmaxf(M, p[(long long)i * SLOT + r]);
     const float b = M == -INFINITY ? 0.f : M;
 #pragma unroll 4
     for (int i = 0; i < splits; ++i) {
-      const float* q = p + (long long)i * C::SLOT;
+      const float* q = p + (long long)i * SLOT;
       const float e = exp2f(q[r] - b);
-      L += q[2 * TQ + r] * e;
-      const float4 u = *reinterpret_cast<const float4*>(q + 4 * TQ + (long long)r * HD + c);
-      const float4 v = *reinterpret_cast<const float4*>(q + 4 * TQ + (long long)r * HD + c + 4);
-      acc[0] += u.x * e; acc[1] += u.y * e; acc[2] += u.z * e; acc[3] += u.w * e;
-      acc[4] += v.x * e; acc[5] += v.y * e; acc[6] += v.z * e; acc[7] += v.w * e;
+      L += q[ROWS + r] * e;
+#pragma unroll
+      for (int k = 0; k < V; k += 4) {
+        const float4 u = *reinterpret_cast<const float4*>(q + 2 * ROWS + (long long)r * HD + c + k);
+        acc[k] += u.x * e; acc[k + 1] += u.y * e; acc[k + 2] += u.z * e; acc[k + 3] += u.w * e;
+      }
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) acc[i] *= inv;
+    for (int i = 0; i < V; ++i) acc[i] *= inv;
     store_vec(static_cast<T*>(a.out) + (rt.r0 + f / a.group) * a.o_row + (long long)(kvh * a.group + f % a.group) * a.o_head + c, acc);
   }
 }
@@ -622,37 +628,46 @@ static bool query_map(CUtensorMap* map, const AttnArgs& a, bool half, int hd) {
 
 // Whether the kernel was built with the registers that its split adds up to.
 template <auto KERN>
-static cudaError_t check_register_split(int dev) {
+static cudaError_t check_register_split(int dev, int threads, int sum) {
   static std::atomic<int> known[VTB_MAX_DEVICES];
   if (known[dev].load(std::memory_order_relaxed)) return cudaSuccess;
   cudaFuncAttributes f;
   const cudaError_t e = cudaFuncGetAttributes(&f, KERN);
   if (e) return e;
-  if (f.numRegs / 8 * 8 * TC_THREADS < 256 * REGS_SOFTMAX + 128 * REGS_OTHER) return cudaErrorInvalidConfiguration;
+  if (f.numRegs / 8 * 8 * threads < sum) return cudaErrorInvalidConfiguration;
   known[dev].store(1, std::memory_order_relaxed);
   return cudaSuccess;
+}
+
+// Query rows of a tile of up to `rows` (whole tokens), and a positive scale.
+static void set_tile(AttnArgs& a, int rows) {
+  a.tile = rows / a.group * a.group;
+  a.recip = 65536 / a.group + 1;
+  a.negate = a.scale2 < 0.f;
+  a.scale2 = fmaxf(fabsf(a.scale2), 1e-36f);  // not 0: masked scores have to stay -inf
+}
+// Fewer items than SMs: the positions are split too, down to two tiles of
+// positions per CTA (below that the join costs more than the split gives).
+static int prefill_splits(const AttnArgs& a, long long units, int tile, int sms) {
+  const long long cap = (long long)a.kv.pages_per_seq << a.kv.page_shift;
+  long long seen = a.window ? (long long)a.window + a.sinks + a.rows : cap;
+  if (seen > cap) seen = cap;
+  long long splits = sms / units;
+  if (splits > seen / (2 * tile)) splits = seen / (2 * tile);
+  return splits > 1 ? (int)splits : 1;
 }
 
 template <typename T, int HD>
 static cudaError_t launch_prefill_tc_t(AttnArgs a, cudaStream_t st) {
   using C = TcPrefill<HD>;
-  a.negate = a.scale2 < 0.f;
-  a.scale2 = fmaxf(fabsf(a.scale2), 1e-36f);  // not 0: masked scores have to stay -inf
   const int dev = current_device();
   cudaError_t e = ensure_smem_attr<paged_prefill_tc_kernel<T, HD>>(dev, C::SMEM);
-  if (e || (e = check_register_split<paged_prefill_tc_kernel<T, HD>>(dev))) return e;
-  a.tile = TQ / a.group * a.group;  // whole tokens
-  a.recip = 65536 / a.group + 1;
+  if (e || (e = check_register_split<paged_prefill_tc_kernel<T, HD>>(dev, TC_THREADS, 256 * REGS_SOFTMAX + 128 * REGS_OTHER)))
+    return e;
+  set_tile(a, TQ);
   const long long units = ((long long)a.rows * a.group / (2 * a.tile) + a.kv.n_seqs) * a.n_kv;
   if (units > 0x7fffffffll / 16) return cudaErrorInvalidValue;
-  // Fewer row tiles than SMs: the positions are split too, down to two tiles of
-  // positions per CTA (below that the join costs more than the split gives).
-  const long long cap = (long long)a.kv.pages_per_seq << a.kv.page_shift;
-  long long seen = a.window ? (long long)a.window + a.sinks + a.rows : cap;
-  if (seen > cap) seen = cap;
-  long long splits = sm_count(dev) / units, most = seen / (2 * TN);
-  if (splits > most) splits = most;
-  if (splits < 1) splits = 1;
+  const int splits = prefill_splits(a, units, TN, sm_count(dev));
   CUtensorMap map_k = {}, map_v = {};
   const int slots = 1 << a.kv.page_shift, fit = slots < TN ? slots : TN;
   CUtensorMap map_q = {};
@@ -661,9 +676,9 @@ static cudaError_t launch_prefill_tc_t(AttnArgs a, cudaStream_t st) {
                           page_map(&map_v, a.kv, a.kv.v, std::is_same<T, __half>::value, HD, a.n_kv, fit) ? fit : 0;
   const long long items = units * splits;
   const unsigned grid = (unsigned)(items < sm_count(dev) ? items : sm_count(dev));
-  paged_prefill_tc_kernel<T, HD><<<grid, TC_THREADS, C::SMEM, st>>>(a, map_k, map_v, map_q, (int)items, (int)splits, box);
+  paged_prefill_tc_kernel<T, HD><<<grid, TC_THREADS, C::SMEM, st>>>(a, map_k, map_v, map_q, (int)items, splits, box);
   if ((e = cudaGetLastError()) || splits == 1) return e;
-  return launch_dependent(paged_prefill_join_kernel<T, HD>, dim3((unsigned)(units * 16)), dim3(256), 0, st, a, (int)splits);
+  return launch_dependent(paged_prefill_join_kernel<T, HD, 2>, dim3((unsigned)(units * 16)), dim3(256), 0, st, a, splits);
 }
 
 cudaError_t launch_paged_prefill_tc(int type, int head_dim, const AttnArgs& a, cudaStream_t st) {
