@@ -92,9 +92,11 @@ __global__ void __launch_bounds__(F_THREADS, 1) paged_prefill_f32_kernel(const _
   if (warp >= 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(F_REGS_SPLIT));
     const int32_t* table = a.kv.table + rt.s * a.kv.table_stride;
-    // byte offset of the row of index i of the span in the cache (-1: none)
+    // Byte offset of the row of index i of the span in the cache.  Indexes behind the
+    // span get the cache's first row: their loads need no branch (which would make
+    // one wait for the other), and zeros replace the values when they are split.
     auto row_of = [&](int i) -> long long {
-      if (i >= sp.n) return -1;
+      if (i >= sp.n) return 0;
       const int pos = sp.pos(i);
       return page_row(a.kv, __ldg(table + (pos >> a.kv.page_shift)), pos) + kvh * a.kv.head_stride;
     };
@@ -116,7 +118,7 @@ __global__ void __launch_bounds__(F_THREADS, 1) paged_prefill_f32_kernel(const _
 #pragma unroll
         for (int i = 0; i < ROUNDS; ++i) {
           const long long off = __shfl_sync(0xffffffffu, mine, i * RPR + lane / PIECES);
-          x[i] = off < 0 ? make_float4(0.f, 0.f, 0.f, 0.f) : *reinterpret_cast<const float4*>(a.kv.k + off + pc * 16);
+          x[i] = *reinterpret_cast<const float4*>(a.kv.k + off + pc * 16);
         }
       };
       // MMA issuer (warp 4): uniform registers, one elected thread
@@ -128,25 +130,24 @@ __global__ void __launch_bounds__(F_THREADS, 1) paged_prefill_f32_kernel(const _
         ok = ok && warp_wait(b, phase & 1);
         tc_fence_after();
       };
-      if (n > 0) fetch(0);
-      if (warp == 4) wait(&bar.q_full, 0);
-      for (int j = 0; j < n; ++j) {
+      auto split = [&](int j) {  // the fetched rows into the shared tile
         if (j) ok = ok && warp_wait(&bar.k_freed, (j - 1) & 1);
-        if (!ok) break;
+        if (!ok) return;
 #pragma unroll
         for (int i = 0; i < ROUNDS; ++i) {
           const int r = r0 + i * RPR;
           const uint32_t d = sk + (pc >> 3) * (FN * 128) + r * 128 + (((pc & 7) ^ (r & 7)) << 4);
+          const bool live = (j0 + j) * FN + r < sp.n;
           const float v[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
           uint32_t hi[4], lo[4];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) split_tf32(v[c], hi[c], lo[c]);
+          for (int c = 0; c < 4; ++c) split_tf32(live ? v[c] : 0.f, hi[c], lo[c]);
           st4(d, hi);
           st4(d + C::KV, lo);
         }
         landed(&bar.k_full);
-        if (j + 1 < n) fetch(j + 1);
-        if (warp != 4) continue;
+      };
+      auto qk = [&](int j) {
         wait(&bar.k_full, j);
         if (ok && elect_one()) {  // (in order behind the product that reads P of the tile before)
           const uint64_t dk = sw128_desc(sk);
@@ -159,6 +160,8 @@ __global__ void __launch_bounds__(F_THREADS, 1) paged_prefill_f32_kernel(const _
           mma_commit(&bar.k_freed);
         }
         __syncwarp();
+      };
+      auto pv = [&](int j) {
         wait(&bar.v_full, j);
         wait(&bar.p_full, j);
         if (ok && elect_one()) {
@@ -172,7 +175,18 @@ __global__ void __launch_bounds__(F_THREADS, 1) paged_prefill_f32_kernel(const _
           mma_commit(&bar.o_full);
         }
         __syncwarp();
+      };
+      if (n > 0) fetch(0);
+      for (int j = 0; j < n && ok; ++j) {  // warp 4 splits its rows of tile j while the softmax of tile j - 1 runs
+        split(j);
+        if (warp == 4) {
+          if (j) pv(j - 1);
+          else wait(&bar.q_full, 0);
+          qk(j);
+        }
+        if (j + 1 < n) fetch(j + 1);
       }
+      if (warp == 4 && n > 0) pv(n - 1);
     } else {
       // ---------------- V: one head dimension per thread, POS positions of it ----------------
       constexpr int POS = FN * HD / 128;
@@ -186,7 +200,7 @@ __global__ void __launch_bounds__(F_THREADS, 1) paged_prefill_f32_kernel(const _
 #pragma unroll
         for (int i = 0; i < POS; ++i) {
           const long long off = __shfl_sync(0xffffffffu, mine[i / 32], i % 32);
-          x[i] = off < 0 ? 0.f : *reinterpret_cast<const float*>(a.kv.v + off + d * 4);
+          x[i] = *reinterpret_cast<const float*>(a.kv.v + off + d * 4);
         }
       };
       if (n > 0) fetch(0);
@@ -199,7 +213,7 @@ __global__ void __launch_bounds__(F_THREADS, 1) paged_prefill_f32_kernel(const _
           const uint32_t at = sv + (pc >> 3) * (HD * 128) + d * 128 + (((pc & 7) ^ (d & 7)) << 4);
           uint32_t hi[4], lo[4];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) split_tf32(x[i + c], hi[c], lo[c]);
+          for (int c = 0; c < 4; ++c) split_tf32((j0 + j) * FN + p0 + i + c < sp.n ? x[i + c] : 0.f, hi[c], lo[c]);
           st4(at, hi);
           st4(at + C::KV, lo);
         }
