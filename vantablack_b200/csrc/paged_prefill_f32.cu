@@ -283,10 +283,15 @@ __global__ void __launch_bounds__(F_THREADS, 1) paged_prefill_f32_kernel(const _
       }
     };
     for (int j = 0; j < n; ++j) {
+      if (j) {  // the last tile's product, while this tile's S is computed
+        ok = warp_wait(&bar.o_full, (j - 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        take();
+      }
       ok = warp_wait(&bar.s_full, j & 1);
       if (!ok) break;
       tc_fence_after();
-      if (j) take();  // complete: this S was issued behind it
       uint32_t s[FN];
       tmem_ld32(s, lanes + C::S);
       tmem_ld32(s + 32, lanes + C::S + 32);
@@ -310,7 +315,7 @@ __global__ void __launch_bounds__(F_THREADS, 1) paged_prefill_f32_kernel(const _
 #pragma unroll
         for (int q = 0; q < 2; ++q) mx[q] = max3(mx[q], __uint_as_float(s[i + 2 * q]), __uint_as_float(s[i + 2 * q + 1]));
       const float mn = fmaxf(m, fmaxf(mx[0], mx[1]) * a.scale2), b = mn == -INFINITY ? 0.f : mn;
-      f = exp2f(m - b);
+      f = ex2(m - b);
       m = mn;
       float sum[2] = {0.f, 0.f};
 #pragma unroll
@@ -318,7 +323,7 @@ __global__ void __launch_bounds__(F_THREADS, 1) paged_prefill_f32_kernel(const _
         uint32_t lo[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-          const float p = exp2f(fmaf(__uint_as_float(s[c + i]), a.scale2, -b));
+          const float p = ex2(fmaf(__uint_as_float(s[c + i]), a.scale2, -b));
           sum[i & 1] += p;
           split_tf32(p, s[c + i], lo[i]);
         }
