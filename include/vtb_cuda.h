@@ -381,6 +381,29 @@ int vtb_cuda_model_set_q8_activations(VtbCudaModel *m, int on);
  * max_rows rows per step (prefill chunk size). */
 VtbCudaState *vtb_cuda_state_create(VtbCudaModel *m, int32_t n_seqs, int32_t max_rows);
 void vtb_cuda_state_destroy(VtbCudaState *s);
+/* A state whose cache is paged: n_pages pages of page_size positions (a power of
+ * two, at most 1024) in kv_type (F32, F16 or BF16), taken by the sequences as
+ * they grow (each at most the model's max_seq positions) and given back on
+ * release or reset.  window > 0: every query sees its sequence's last `window`
+ * positions and its first `sinks`, and pages left behind by the window are given
+ * back.  head_dim 64 or 128, one GPU.  Every call on states works on it; a step
+ * or prefill that finds no free page fails with -7 before it changes anything
+ * (vtb_cuda_prefill in chunks of max_rows: before the chunk that finds none). */
+typedef struct VtbCudaPagedConfig {
+  int32_t page_size, n_pages, kv_type, window, sinks;
+} VtbCudaPagedConfig;
+VtbCudaState *vtb_cuda_state_create_paged(VtbCudaModel *m, int32_t n_seqs, int32_t max_rows,
+                                          const VtbCudaPagedConfig *cfg);
+/* Sequence dst becomes a copy of sequence src (whose position it takes over): whole
+ * pages are shared between them, a page that src has begun is copied. */
+int vtb_cuda_state_fork(VtbCudaState *s, int32_t dst, int32_t src);
+/* Gives back the pages of sequence seq and sets its position to 0. */
+int vtb_cuda_state_release(VtbCudaState *s, int32_t seq);
+/* Pages that no sequence holds (-1: not a paged state). */
+int64_t vtb_cuda_state_free_pages(const VtbCudaState *s);
+/* Moves the pages in use to the front of the pool; returns their number (negative:
+ * a status). */
+int64_t vtb_cuda_state_compact(VtbCudaState *s);
 /* KvCache.reset (kv_cache.zig:80). */
 int vtb_cuda_state_reset(VtbCudaState *s);
 /* KvCache.pos of sequence `seq` (host-authoritative). */

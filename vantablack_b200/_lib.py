@@ -75,6 +75,11 @@ SIGNATURES = {
     "vtb_cuda_model_weight_bytes": (_sz, [_vp]),
     "vtb_cuda_model_set_q8_activations": (_int, [_vp, _int]),
     "vtb_cuda_state_create": (_vp, [_vp, _i32, _i32]),
+    "vtb_cuda_state_create_paged": (_vp, [_vp, _i32, _i32, _vp]),
+    "vtb_cuda_state_fork": (_int, [_vp, _i32, _i32]),
+    "vtb_cuda_state_release": (_int, [_vp, _i32]),
+    "vtb_cuda_state_free_pages": (_i64, [_vp]),
+    "vtb_cuda_state_compact": (_i64, [_vp]),
     "vtb_cuda_state_destroy": (None, [_vp]),
     "vtb_cuda_state_reset": (_int, [_vp]),
     "vtb_cuda_state_pos": (_i64, [_vp, _i32]),
@@ -139,6 +144,11 @@ class PagedAttn(C.Structure):
     _fields_ = [("q", _vp), ("out", _vp), ("q_row_stride", _i64), ("q_head_stride", _i64), ("out_row_stride", _i64),
                 ("out_head_stride", _i64), ("n_heads", _i32), ("window", _i32), ("sinks", _i32), ("scale", C.c_float),
                 ("lens", _vp), ("workspace", _vp), ("workspace_bytes", _sz)]
+
+
+class PagedConfig(C.Structure):
+    """VtbCudaPagedConfig."""
+    _fields_ = [("page_size", _i32), ("n_pages", _i32), ("kv_type", _i32), ("window", _i32), ("sinks", _i32)]
 
 
 class VtbError(RuntimeError):

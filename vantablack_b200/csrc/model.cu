@@ -52,6 +52,13 @@ __global__ void add_kernel(float* __restrict__ x, const float* __restrict__ t, l
     x[i] += t[i];
 }
 
+// Attention output of a 16-bit paged cache for the f32 projections.
+template <typename T>
+__global__ void widen_kernel(const T* __restrict__ x, float* __restrict__ y, long long n) {
+  const long long i = blockIdx.x * (long long)blockDim.x + threadIdx.x;
+  if (i < n) y[i] = to_f(x[i]);
+}
+
 cudaError_t launch_gemv_q8_0_q8_0(const void* w, const int8_t* xq, const float* dx, float* y, int m, int k,
                                   cudaStream_t st, bool pdl, int accumulate);
 cudaError_t launch_quantize_q8_0(const float* x, int8_t* qs, float* d, int nblocks, cudaStream_t st);
@@ -863,6 +870,31 @@ struct VtbCudaModel {
   bool q8_act = false;
 };
 
+// Pages of a paged state: which are taken, by how many sequences, and where the
+// cache lies.  The table is kept on the host and goes to the device when a step
+// has changed it.
+struct PagePool {
+  VtbCudaPagedConfig c;
+  int n_seqs, per;               // sequences, pages per sequence
+  std::vector<int32_t> refs;     // sequences that hold each page
+  std::vector<int32_t> free_ids; // pages that none holds (taken from the back)
+  std::vector<int32_t> first;    // per sequence: pages behind the sinks that the window has left
+  int32_t* table = nullptr;      // pinned [n_seqs][per], -1: no page
+  int32_t* d_table = nullptr;
+  bool dirty = true;
+  char* k = nullptr;             // [n_layers][n_pages][n_kv][page_size][head_dim]
+  char* v = nullptr;
+  size_t layer_elems = 0;
+  void* q = nullptr;             // [rows][H][head_dim] rotated queries in the cache's type
+  void* out = nullptr;           // attention output of a 16-bit cache
+  void* ws = nullptr;
+  size_t ws_bytes = 0;
+  int32_t* lists = nullptr;      // pinned and device: src | dst | map of a copy, [3][n_pages]
+  int32_t* d_lists = nullptr;
+  int32_t* lens = nullptr;       // device [n_seqs], and starts [n_seqs + 1] behind it
+  int32_t& at(int s, int i) { return table[(size_t)s * per + i]; }
+};
+
 struct VtbCudaState {
   VtbCudaModel* m;
   int device;  // kept here so destroy never touches the model
@@ -895,6 +927,7 @@ struct VtbCudaState {
   int tp_rank = 0;
   long long flag_off = 0;   // floats from a block's start to its flags
   int par = 0;              // slot of the next all-reduce (host count mod 2; every call does an even number)
+  PagePool* pool = nullptr; // paged cache (vtb_cuda_state_create_paged) in place of kc / vc
 };
 
 // Error text goes to the same thread-local buffer as the rest of the shim
@@ -1176,7 +1209,100 @@ int vtb_cuda_model_set_q8_activations(VtbCudaModel* m, int on) {
   return VTB_CUDA_OK;
 }
 
-VtbCudaState* vtb_cuda_state_create(VtbCudaModel* m, int32_t n_seqs, int32_t max_rows) {
+// Takes a page for position `pos` of sequence s if it has none there.
+static bool pool_take(PagePool* p, int s, int pos) {
+  int32_t& e = p->at(s, pos / p->c.page_size);
+  if (e >= 0) return true;
+  if (p->free_ids.empty()) return false;
+  e = p->free_ids.back();
+  p->free_ids.pop_back();
+  p->refs[e] = 1;
+  p->dirty = true;
+  return true;
+}
+static void pool_drop(PagePool* p, int32_t& e) {
+  if (e < 0) return;
+  if (--p->refs[e] == 0) p->free_ids.push_back(e);
+  e = -1;
+  p->dirty = true;
+}
+static void pool_drop_seq(PagePool* p, int s) {
+  for (int i = 0; i < p->per; ++i) pool_drop(p, p->at(s, i));
+  p->first[s] = 0;
+}
+// Gives back the pages of sequence s that no query at `pos` or later sees.
+static void pool_evict(PagePool* p, int s, int64_t pos) {
+  if (!p->c.window) return;
+  const int ps = p->c.page_size, keep = (p->c.sinks + ps - 1) / ps;
+  int& i = p->first[s];
+  if (i < keep) i = keep;
+  for (; (int64_t)(i + 1) * ps <= pos + 1 - p->c.window; ++i) pool_drop(p, p->at(s, i));
+}
+// Pages for a step's rows, all or none.
+static int pool_reserve(PagePool* p, int rows, const int32_t* seq, const int32_t* pos) {
+  std::vector<int32_t*> taken;
+  for (int r = 0; r < rows; ++r) {
+    int32_t& e = p->at(seq[r], pos[r] / p->c.page_size);
+    if (e >= 0) continue;
+    if (!pool_take(p, seq[r], pos[r])) {
+      for (int32_t* t : taken) pool_drop(p, *t);
+      return merr(VTB_CUDA_ERR_STREAM_ABORTED, "KV cache pages exhausted");
+    }
+    taken.push_back(&e);
+  }
+  return VTB_CUDA_OK;
+}
+static void pool_free(PagePool* p) {
+  if (!p) return;
+  cudaFreeHost(p->table);
+  cudaFreeHost(p->lists);
+  cudaFree(p->d_table);
+  cudaFree(p->d_lists);
+  cudaFree(p->k);
+  cudaFree(p->v);
+  cudaFree(p->q);
+  cudaFree(p->out);
+  cudaFree(p->ws);
+  delete p;
+}
+static VtbCudaPagedKv pool_view(const PagePool* p, const VtbCudaModel* m, int layer) {
+  const int es = p->c.kv_type == F32 ? 4 : 2, hd = m->c.head_dim;
+  const size_t off = (size_t)layer * p->layer_elems * es;
+  return VtbCudaPagedKv{p->k + off, p->v + off, p->c.kv_type, m->KV, hd, p->c.page_size, p->c.n_pages,
+                        (int64_t)m->KV * p->c.page_size * hd, (int64_t)p->c.page_size * hd, hd, p->d_table, p->per,
+                        p->n_seqs, p->per};
+}
+static PagePool* pool_create(VtbCudaModel* m, int n_seqs, int max_rows, const VtbCudaPagedConfig* pc, cudaStream_t st) {
+  const VtbCudaLlamaConfig& c = m->c;
+  PagePool* p = new (std::nothrow) PagePool();
+  if (!p) return nullptr;
+  p->c = *pc;
+  p->n_seqs = n_seqs;
+  p->per = (c.max_seq + pc->page_size - 1) / pc->page_size;
+  const size_t es = pc->kv_type == F32 ? 4 : 2, rows = (size_t)max_rows * m->H * c.head_dim;
+  p->layer_elems = (size_t)pc->n_pages * m->KV * pc->page_size * c.head_dim;
+  const size_t kv = p->layer_elems * c.n_layers * es, tab = (size_t)n_seqs * p->per * 4, lists = (size_t)3 * pc->n_pages * 4;
+  p->ws_bytes = vtb_cuda_paged_attn_workspace_bytes(pc->kv_type, m->H, m->KV, c.head_dim);
+  if (cudaMallocHost(&p->table, tab) != cudaSuccess || cudaMallocHost(&p->lists, lists) != cudaSuccess ||
+      cudaMalloc(&p->d_table, tab) != cudaSuccess || cudaMalloc(&p->d_lists, lists) != cudaSuccess ||
+      cudaMalloc(&p->k, kv) != cudaSuccess || cudaMalloc(&p->v, kv) != cudaSuccess ||
+      cudaMalloc(&p->q, rows * es) != cudaSuccess || (es == 2 && cudaMalloc(&p->out, rows * es) != cudaSuccess) ||
+      cudaMalloc(&p->ws, p->ws_bytes) != cudaSuccess) {
+    cudaGetLastError();
+    merr(VTB_CUDA_ERR_OOM, "state: out of memory (KV pages)");
+    pool_free(p);
+    return nullptr;
+  }
+  cudaMemsetAsync(p->k, 0, kv, st);
+  cudaMemsetAsync(p->v, 0, kv, st);
+  std::fill(p->table, p->table + tab / 4, -1);
+  p->refs.assign(pc->n_pages, 0);
+  p->first.assign(n_seqs, 0);
+  for (int i = pc->n_pages - 1; i >= 0; --i) p->free_ids.push_back(i);
+  return p;
+}
+
+static VtbCudaState* state_create(VtbCudaModel* m, int32_t n_seqs, int32_t max_rows, const VtbCudaPagedConfig* pc) {
   if (!m || n_seqs <= 0 || max_rows < n_seqs || max_rows > 65535) {
     merr(VTB_CUDA_ERR_INVALID_ARG, "bad state dimensions");
     return nullptr;
@@ -1216,19 +1342,20 @@ VtbCudaState* vtb_cuda_state_create(VtbCudaModel* m, int32_t n_seqs, int32_t max
       return nullptr;
     }
   }
-  s->nsplit = (c.max_seq + DEC_CHUNK - 1) / DEC_CHUNK;
+  s->nsplit = pc ? 1 : (c.max_seq + DEC_CHUNK - 1) / DEC_CHUNK;  // (a paged state's partials live in its workspace)
   const size_t R = max_rows, d = c.dim, hd = c.head_dim, qd = (size_t)m->H * hd, kvd = (size_t)m->KV * hd, f = m->F;
   const size_t qkvw = qd + 2 * kvd;
   const size_t kmax = d > f ? d : f;
   // split-K partials for small-batch GEMMs: splits x rows <= 512 of the widest projection
   const size_t gsplit = R >= (size_t)GEMM_MIN_ROWS ? 512 * std::max(std::max(qkvw, 2 * f), d) : 0;
   size_t fl = R * (d + d + qkvw + qd + 2 * f + f + (size_t)c.vocab_size + m->V + d + kmax) +
-              R * m->H * (size_t)s->nsplit * (hd + 2) + gsplit + (size_t)c.max_seq * hd + 64;
-  const size_t kvn = (size_t)n_seqs * c.n_layers * c.max_seq * kvd;
+              R * (m->H * (size_t)s->nsplit * (hd + 2) + 2 * ARGMAX_PARTS) + gsplit + (size_t)c.max_seq * hd + 64;
+  const size_t kvn = pc ? 0 : (size_t)n_seqs * c.n_layers * c.max_seq * kvd;
+  const size_t extra = pc ? 2 * (size_t)n_seqs + 1 : 0;  // lens | starts, behind tok | seq | pos
   float* base = nullptr;
   int32_t* ib = nullptr;
-  if (cudaMalloc(&base, (fl + 2 * kvn) * 4 + 64) != cudaSuccess || cudaMalloc(&ib, 4 * R * 4) != cudaSuccess ||
-      cudaMallocHost(&s->hbuf, 3 * R * 4) != cudaSuccess || cudaMallocHost(&s->hamax, R * 4) != cudaSuccess) {
+  if (cudaMalloc(&base, (fl + 2 * kvn) * 4 + 64) != cudaSuccess || cudaMalloc(&ib, (4 * R + extra) * 4) != cudaSuccess ||
+      cudaMallocHost(&s->hbuf, (3 * R + extra) * 4) != cudaSuccess || cudaMallocHost(&s->hamax, R * 4) != cudaSuccess) {
     cudaGetLastError();
     cudaFree(base);
     cudaFree(ib);
@@ -1241,14 +1368,22 @@ VtbCudaState* vtb_cuda_state_create(VtbCudaModel* m, int32_t n_seqs, int32_t max
   s->x = carve(R * d); s->xb = carve(R * d); s->qkv = carve(R * qkvw); s->att = carve(R * qd);
   s->gu = carve(R * 2 * f); s->h = carve(R * f); s->logits = carve(R * c.vocab_size);
   s->logits_local = carve(R * m->V);
-  s->part = carve(R * m->H * (size_t)s->nsplit * (hd + 2));
+  s->part = carve(R * (m->H * (size_t)s->nsplit * (hd + 2) + 2 * ARGMAX_PARTS));
   s->tmp = carve(R * d);
   s->ws = carve(R * kmax);  // bf16 hi + lo = 4 bytes per activation
   s->gsplit = gsplit ? carve(gsplit) : nullptr;
   s->gsplit_elems = gsplit;
   s->kc = carve(kvn); s->vc = carve(kvn);
   s->rope = carve((size_t)c.max_seq * hd);
-  s->tok = ib; s->seq = ib + R; s->pos = ib + 2 * R; s->amax = ib + 3 * R;
+  s->tok = ib; s->seq = ib + R; s->pos = ib + 2 * R; s->amax = ib + 3 * R + extra;
+  if (pc) {
+    s->pool = pool_create(m, n_seqs, max_rows, pc, s->st);
+    if (!s->pool) {
+      vtb_cuda_state_destroy(s);
+      return nullptr;
+    }
+    s->pool->lens = ib + 3 * R;
+  }
   cudaMemsetAsync(s->kc, 0, 2 * kvn * 4, s->st);
   // RoPE angles with the reference's float steps (math.zig:88-104): inv_freq =
   // 1 / pow(base, i / hd), theta = pos * inv_freq, cos / sin, computed once on
@@ -1274,12 +1409,117 @@ VtbCudaState* vtb_cuda_state_create(VtbCudaModel* m, int32_t n_seqs, int32_t max
   return s;
 }
 
+VtbCudaState* vtb_cuda_state_create(VtbCudaModel* m, int32_t n_seqs, int32_t max_rows) {
+  return state_create(m, n_seqs, max_rows, nullptr);
+}
+
+VtbCudaState* vtb_cuda_state_create_paged(VtbCudaModel* m, int32_t n_seqs, int32_t max_rows, const VtbCudaPagedConfig* pc) {
+  cudaGetLastError();
+  int status = VTB_CUDA_OK;
+  if (!m || !pc || pc->page_size < 1 || pc->page_size > 1024 || (pc->page_size & (pc->page_size - 1)) || pc->n_pages < 1 ||
+      pc->window < 0 || pc->sinks < 0 || (pc->sinks && !pc->window))
+    status = merr(VTB_CUDA_ERR_INVALID_ARG, "bad paged state configuration");
+  else if (pc->kv_type != F32 && pc->kv_type != T_F16 && pc->kv_type != T_BF16)
+    status = merr(VTB_CUDA_ERR_UNSUPPORTED, "cache type must be F32, F16 or BF16");
+  else if ((m->c.head_dim != 64 && m->c.head_dim != 128) || (m->tp && m->tp->world > 1))
+    status = merr(VTB_CUDA_ERR_UNSUPPORTED, "paged states need head_dim 64 or 128 and one GPU");
+  return status ? nullptr : state_create(m, n_seqs, max_rows, pc);
+}
+
+// Pages of sequence `src` for `dst` too: whole pages are shared, the last one, which
+// both will go on writing, is copied.
+int vtb_cuda_state_fork(VtbCudaState* s, int32_t dst, int32_t src) {
+  cudaGetLastError();
+  if (!s || !s->pool || dst < 0 || src < 0 || dst >= s->n_seqs || src >= s->n_seqs || dst == src)
+    return merr(VTB_CUDA_ERR_INVALID_ARG, "bad fork arguments");
+  if (s->rows > 0) return merr(VTB_CUDA_ERR_INVALID_ARG, "a token is being computed (vtb_cuda_finalize_token ends it)");
+  cudaSetDevice(s->device);
+  PagePool* p = s->pool;
+  const int64_t pos = s->seq_pos[src];
+  const int last = (int)(pos / p->c.page_size);
+  const bool tail = pos % p->c.page_size != 0;
+  // The page for the copy is found before anything changes: a free one, or one that only dst holds.
+  if (tail && p->free_ids.empty()) {
+    bool gives = false;
+    for (int i = 0; i < p->per && !gives; ++i) gives = p->at(dst, i) >= 0 && p->refs[p->at(dst, i)] == 1;
+    if (!gives) return merr(VTB_CUDA_ERR_STREAM_ABORTED, "KV cache pages exhausted");
+  }
+  pool_drop_seq(p, dst);
+  for (int i = 0; i < p->per; ++i) {
+    const int32_t e = p->at(src, i);
+    if (e < 0 || (tail && i == last)) continue;
+    p->at(dst, i) = e;
+    ++p->refs[e];
+  }
+  p->first[dst] = p->first[src];
+  p->dirty = true;
+  s->seq_pos[dst] = pos;
+  if (!tail) return VTB_CUDA_OK;
+  pool_take(p, dst, (int)pos);
+  p->lists[0] = p->at(src, last);
+  p->lists[1] = p->at(dst, last);
+  cudaError_t e = cudaMemcpyAsync(p->d_lists, p->lists, 8, cudaMemcpyHostToDevice, s->st);
+  if (e != cudaSuccess) return mcuda(e);
+  const VtbCudaPagedKv kv = pool_view(p, s->m, 0);
+  const int rc = vtb_cuda_paged_copy(&kv, s->m->c.n_layers, (int64_t)p->layer_elems, p->d_lists, p->d_lists + 1, 1, nullptr, nullptr, s->st);
+  return rc ? rc : mcuda(cudaStreamSynchronize(s->st));  // (the lists are free again)
+}
+
+int vtb_cuda_state_release(VtbCudaState* s, int32_t seq) {
+  if (!s || !s->pool || seq < 0 || seq >= s->n_seqs) return merr(VTB_CUDA_ERR_INVALID_ARG, "bad release arguments");
+  if (s->rows > 0) return merr(VTB_CUDA_ERR_INVALID_ARG, "a token is being computed (vtb_cuda_finalize_token ends it)");
+  pool_drop_seq(s->pool, seq);
+  s->seq_pos[seq] = 0;
+  return VTB_CUDA_OK;
+}
+
+int64_t vtb_cuda_state_free_pages(const VtbCudaState* s) { return s && s->pool ? (int64_t)s->pool->free_ids.size() : -1; }
+
+// Live pages behind the first n (n: how many live) move into the holes before them.
+int64_t vtb_cuda_state_compact(VtbCudaState* s) {
+  cudaGetLastError();
+  if (!s || !s->pool) return merr(VTB_CUDA_ERR_INVALID_ARG, "not a paged state");
+  if (s->rows > 0) return merr(VTB_CUDA_ERR_INVALID_ARG, "a token is being computed (vtb_cuda_finalize_token ends it)");
+  cudaSetDevice(s->device);
+  PagePool* p = s->pool;
+  const int n_pages = p->c.n_pages, live = n_pages - (int)p->free_ids.size();
+  int32_t *src = p->lists, *dst = src + n_pages, *map = dst + n_pages;
+  int n = 0, hole = 0;
+  for (int i = 0; i < n_pages; ++i) map[i] = i;
+  for (int i = live; i < n_pages; ++i) {
+    if (!p->refs[i]) continue;
+    while (p->refs[hole]) ++hole;
+    src[n] = i;
+    dst[n++] = hole;
+    map[i] = hole;
+    p->refs[hole] = p->refs[i];
+    p->refs[i] = 0;
+  }
+  if (n == 0) return live;
+  cudaError_t e = cudaMemcpyAsync(p->d_lists, p->lists, (size_t)3 * n_pages * 4, cudaMemcpyHostToDevice, s->st);
+  if (e == cudaSuccess && p->dirty)
+    e = cudaMemcpyAsync(p->d_table, p->table, (size_t)p->n_seqs * p->per * 4, cudaMemcpyHostToDevice, s->st);
+  if (e != cudaSuccess) return mcuda(e);
+  const VtbCudaPagedKv kv = pool_view(p, s->m, 0);
+  const int rc = vtb_cuda_paged_copy(&kv, s->m->c.n_layers, (int64_t)p->layer_elems, p->d_lists, p->d_lists + n_pages, n, p->d_table,
+                                     p->d_lists + 2 * n_pages, s->st);
+  if (rc) return rc;
+  if ((e = cudaStreamSynchronize(s->st)) != cudaSuccess) return mcuda(e);
+  for (size_t i = 0; i < (size_t)p->n_seqs * p->per; ++i)
+    if (p->table[i] >= 0) p->table[i] = map[p->table[i]];
+  p->free_ids.clear();
+  for (int i = n_pages - 1; i >= live; --i) p->free_ids.push_back(i);
+  p->dirty = false;
+  return live;
+}
+
 void vtb_cuda_state_destroy(VtbCudaState* s) {
   if (!s) return;
   cudaSetDevice(s->device);
   cudaStreamSynchronize(s->st);
   if (s->graph) cudaGraphExecDestroy(s->graph);
   tp_p2p_release(s);
+  pool_free(s->pool);
   cudaStreamDestroy(s->st);
   cudaFree(s->x);
   cudaFree(s->tok);
@@ -1291,6 +1531,13 @@ void vtb_cuda_state_destroy(VtbCudaState* s) {
 int vtb_cuda_state_reset(VtbCudaState* s) {
   if (!s) return merr(VTB_CUDA_ERR_INVALID_ARG, "null state");
   for (auto& p : s->seq_pos) p = 0;
+  if (s->pool) {
+    cudaSetDevice(s->device);
+    const cudaError_t e = cudaStreamSynchronize(s->st);  // a token being computed reads the table
+    if (e != cudaSuccess) return mcuda(e);
+    s->rows = 0;
+    for (int q = 0; q < s->n_seqs; ++q) pool_drop_seq(s->pool, q);
+  }
   return VTB_CUDA_OK;
 }
 
@@ -1323,6 +1570,21 @@ static int stage_rows(VtbCudaState* s, int rows, const int32_t* tok, const int32
   for (int r = 0; r < rows; ++r) s->max_pos = std::max(s->max_pos, (int)pos[r]);
   s->one_seq = true;
   for (int r = 1; r < rows; ++r) s->one_seq = s->one_seq && seq[r] == seq[0];
+  if (PagePool* p = s->pool) {
+    // rows are one token of each sequence in order (decode), or consecutive tokens of one (prefill)
+    int rc = pool_reserve(p, rows, seq, pos);
+    if (rc) {
+      s->rows = 0;
+      return rc;
+    }
+    int32_t *lens = s->hbuf + 3 * (size_t)s->max_rows, *starts = lens + s->n_seqs;
+    for (int q = 0, r = 0; q < s->n_seqs; ++q) {
+      lens[q] = (int32_t)s->seq_pos[q];
+      starts[q] = r;
+      for (; r < rows && seq[r] == q; ++r) lens[q] = pos[r] + 1;
+    }
+    starts[s->n_seqs] = rows;
+  }
   s->decode_rows = true;
   for (int r = 1; r < rows && s->decode_rows; ++r)
     for (int q = 0; q < r; ++q)
@@ -1330,9 +1592,19 @@ static int stage_rows(VtbCudaState* s, int rows, const int32_t* tok, const int32
   return VTB_CUDA_OK;
 }
 
+// The page table, when a step has changed it (outside of a captured step, whose
+// kernels read it where it lies).
+static cudaError_t upload_table(VtbCudaState* s) {
+  PagePool* p = s->pool;
+  if (!p || !p->dirty) return cudaSuccess;
+  p->dirty = false;
+  return cudaMemcpyAsync(p->d_table, p->table, (size_t)p->n_seqs * p->per * 4, cudaMemcpyHostToDevice, s->st);
+}
+
 static cudaError_t enqueue_embed(VtbCudaState* s) {
   const int R = s->max_rows;
-  cudaError_t e = cudaMemcpyAsync(s->tok, s->hbuf, 3 * R * 4, cudaMemcpyHostToDevice, s->st);
+  const size_t extra = s->pool ? 2 * (size_t)s->n_seqs + 1 : 0;
+  cudaError_t e = cudaMemcpyAsync(s->tok, s->hbuf, (3 * (size_t)R + extra) * 4, cudaMemcpyHostToDevice, s->st);
   if (e != cudaSuccess) return e;
   return launch_embed(s->m->q_embd, s->m->embd, s->tok, s->x, s->m->c.dim, s->rows, s->st);
 }
@@ -1462,6 +1734,34 @@ static cudaError_t enqueue_layer(VtbCudaState* s, int l) {
     return allreduce_tmp(s, (size_t)R * d);
   };
   e = cudaSuccess;
+  // The second half of the block: FFN RMSNorm, gate|up, SwiGLU, down (forward.zig:276-287).
+  auto enqueue_ffn = [&]() -> cudaError_t {
+    if (!gemm && L.gu && L.gu_il && L.q_gate == Q4_K) {
+      // SwiGLU in the GEMV's epilogue (h directly); the FFN RMSNorm in its prologue,
+      // or, with a tensor-parallel partial pending, in the all-reduce kernel before it
+      const bool pend = s->pending;
+      if (pend && (e = enqueue_norm(s, L.ffn_norm, 0, R))) return e;
+      for (int r = 0; r < R && e == cudaSuccess; ++r)
+        e = launch_gemv_q4k_mma(L.gu, (pend ? s->xb : s->x) + (size_t)r * d, nullptr, 2 * f, d, st, true, 0,
+                                pend ? nullptr : L.ffn_norm, c.rms_eps, s->h + (size_t)r * f);
+      if (e) return e;
+      return residual(L.q_down, L.down, s->h, f, L.down_pitch);
+    }
+    if (fused_norm_gemv(L.ffn_norm, L.q_gate, L.gu, s->gu, 2 * f)) {
+      if (e) return e;
+    } else if ((e = enqueue_norm(s, L.ffn_norm, 0, R))) {
+      return e;
+    } else if (L.gu) {
+      if ((e = proj(L.q_gate, L.gu, s->xb, s->gu, 2 * f, d, 2 * f, 0))) return e;
+    } else {
+      if ((e = proj(L.q_gate, L.gate, s->xb, s->gu, f, d, 2 * f, 0))) return e;
+      if ((e = proj(L.q_up, L.up, s->xb, s->gu + f, f, d, 2 * f, 0))) return e;
+    }
+    if ((e = pdl_launch(swiglu_kernel, dim3(min(1184, (R * f + 255) / 256)), dim3(256), 0, st, (const float*)s->gu, s->h,
+                        f, R, L.gu && L.gu_il ? 1 : 0)))
+      return e;
+    return residual(L.q_down, L.down, s->h, f, L.down_pitch);
+  };
   if (fused_norm_gemv(L.attn_norm, L.q_q, L.qkv, s->qkv, qkvw)) {
     if (e) return e;
   } else if ((e = enqueue_norm(s, L.attn_norm, 0, R))) {
@@ -1472,6 +1772,25 @@ static cudaError_t enqueue_layer(VtbCudaState* s, int l) {
     if ((e = proj(L.q_q, L.q, s->xb, s->qkv, qd, d, qkvw, 0))) return e;
     if ((e = proj(L.q_k, L.k, s->xb, s->qkv + qd, kvd, d, qkvw, 0))) return e;
     if ((e = proj(L.q_v, L.v, s->xb, s->qkv + qd + kvd, kvd, d, qkvw, 0))) return e;
+  }
+  if (PagePool* p = s->pool) {
+    const VtbCudaPagedKv kv = pool_view(p, m, l);
+    const VtbCudaPagedRows rows{F32, H, R, s->qkv + qd, s->qkv + qd + kvd, s->qkv, qkvw, hd, qkvw, hd, qkvw, hd,
+                                p->q, s->rope, c.max_seq, s->seq, s->pos};
+    const VtbCudaPagedAttn attn{p->q, p->out ? p->out : s->att, qd, hd, qd, hd, H, p->c.window, p->c.sinks,
+                                1.0f / sqrtf((float)hd), p->lens, p->ws, p->ws_bytes};
+    int rc = vtb_cuda_paged_append(&kv, &rows, st);
+    if (!rc) rc = s->decode_rows && R == s->n_seqs ? vtb_cuda_paged_attn_decode(&kv, &attn, st)
+                                                   : vtb_cuda_paged_attn_prefill(&kv, &attn, p->lens + s->n_seqs, R, st);
+    if (rc) return cudaErrorUnknown;
+    if (p->out) {
+      const long long n = (long long)R * qd;
+      if (p->c.kv_type == T_F16) widen_kernel<<<dim3((unsigned)((n + 255) / 256)), 256, 0, st>>>((const __half*)p->out, s->att, n);
+      else widen_kernel<<<dim3((unsigned)((n + 255) / 256)), 256, 0, st>>>((const __nv_bfloat16*)p->out, s->att, n);
+      if ((e = cudaGetLastError())) return e;
+    }
+    if ((e = residual(L.q_o, L.o, s->att, qd, 0))) return e;
+    return enqueue_ffn();
   }
   // Decode rows are distinct sequences: each row's new K/V is read only by its
   // own attention, so RoPE + the cache write fold into the attention kernel.
@@ -1522,31 +1841,7 @@ static cudaError_t enqueue_layer(VtbCudaState* s, int l) {
       return e;
   }
   if ((e = residual(L.q_o, L.o, s->att, qd, 0))) return e;  // x += W_o . att (addInto fused)
-  if (!gemm && L.gu && L.gu_il && L.q_gate == Q4_K) {
-    // SwiGLU in the GEMV's epilogue (h directly); the FFN RMSNorm in its prologue,
-    // or, with a tensor-parallel partial pending, in the all-reduce kernel before it
-    const bool pend = s->pending;
-    if (pend && (e = enqueue_norm(s, L.ffn_norm, 0, R))) return e;
-    for (int r = 0; r < R && e == cudaSuccess; ++r)
-      e = launch_gemv_q4k_mma(L.gu, (pend ? s->xb : s->x) + (size_t)r * d, nullptr, 2 * f, d, st, true, 0,
-                              pend ? nullptr : L.ffn_norm, c.rms_eps, s->h + (size_t)r * f);
-    if (e) return e;
-    return residual(L.q_down, L.down, s->h, f, L.down_pitch);
-  }
-  if (fused_norm_gemv(L.ffn_norm, L.q_gate, L.gu, s->gu, 2 * f)) {
-    if (e) return e;
-  } else if ((e = enqueue_norm(s, L.ffn_norm, 0, R))) {
-    return e;
-  } else if (L.gu) {
-    if ((e = proj(L.q_gate, L.gu, s->xb, s->gu, 2 * f, d, 2 * f, 0))) return e;
-  } else {
-    if ((e = proj(L.q_gate, L.gate, s->xb, s->gu, f, d, 2 * f, 0))) return e;
-    if ((e = proj(L.q_up, L.up, s->xb, s->gu + f, f, d, 2 * f, 0))) return e;
-  }
-  if ((e = pdl_launch(swiglu_kernel, dim3(min(1184, (R * f + 255) / 256)), dim3(256), 0, st, (const float*)s->gu, s->h,
-                      f, R, L.gu && L.gu_il ? 1 : 0)))
-    return e;
-  return residual(L.q_down, L.down, s->h, f, L.down_pitch);
+  return enqueue_ffn();
 }
 
 // Final RMSNorm + LM head (backend_cpu.zig finalStep :88-106) and argmax.
@@ -1611,7 +1906,8 @@ int vtb_cuda_begin_token(VtbCudaState* s, const int32_t* tokens) {
   for (int i = 0; i < s->n_seqs; ++i) { seq[i] = i; pos[i] = (int32_t)s->seq_pos[i]; }
   int rc = stage_rows(s, s->n_seqs, tokens, seq.data(), pos.data());
   if (rc) return rc;
-  return mcuda(enqueue_embed(s));
+  cudaError_t e = upload_table(s);
+  return mcuda(e ? e : enqueue_embed(s));
 }
 
 int vtb_cuda_layer_step(VtbCudaState* s, int32_t layer) {
@@ -1633,7 +1929,10 @@ int vtb_cuda_finalize_token(VtbCudaState* s, float* logits, int32_t* argmax) {
   const int n = s->rows;
   int rc = finalize(s, n, logits, argmax);
   if (rc == VTB_CUDA_OK)  // cache.advance (forward.zig:168)
-    for (int i = 0; i < s->n_seqs; ++i) s->seq_pos[i] += 1;
+    for (int i = 0; i < s->n_seqs; ++i) {
+      s->seq_pos[i] += 1;
+      if (s->pool) pool_evict(s->pool, i, s->seq_pos[i]);
+    }
   s->rows = 0;
   return rc;
 }
@@ -1649,6 +1948,7 @@ int vtb_cuda_step(VtbCudaState* s, const int32_t* tokens, float* logits, int32_t
   for (int i = 0; i < s->n_seqs; ++i) { seq[i] = i; pos[i] = (int32_t)s->seq_pos[i]; }
   int rc = stage_rows(s, s->n_seqs, tokens, seq.data(), pos.data());
   if (rc) return rc;
+  if (cudaError_t et = upload_table(s)) return mcuda(et);
   if (!s->graph || s->graph_rows != s->rows) {
     if (s->graph) { cudaGraphExecDestroy(s->graph); s->graph = nullptr; }
     // Warm the kernels' one-time attribute setup outside of capture.
@@ -1694,13 +1994,19 @@ int vtb_cuda_prefill(VtbCudaState* s, int32_t seq, const int32_t* tokens, int32_
     for (int r = 0; r < rows; ++r) pos[r] = (int32_t)(s->seq_pos[seq] + r);
     int rc = stage_rows(s, rows, tokens + done, sq.data(), pos.data());
     if (rc) return rc;
-    cudaError_t e = enqueue_embed(s);
+    cudaError_t e = upload_table(s);
+    if (e == cudaSuccess) e = enqueue_embed(s);
     for (int l = 0; l < c.n_layers && e == cudaSuccess; ++l) e = enqueue_layer(s, l);
     const bool last = done + rows == n;
     if (e == cudaSuccess && last) e = enqueue_final(s, true);
     if (e != cudaSuccess) return mcuda(e);
     s->seq_pos[seq] += rows;
     done += rows;
+    if (s->pool) {
+      // the next chunk's staging and table may change only when this one has been read
+      if (!last && (e = cudaStreamSynchronize(s->st))) return mcuda(e);
+      pool_evict(s->pool, seq, s->seq_pos[seq]);
+    }
     if (last) {
       s->rows = 1;
       rc = finalize(s, 1, logits, argmax);

@@ -311,15 +311,32 @@ class CudaModel:
             pass
 
 
+@dataclass
+class PagedConfig:
+    """A paged KV cache (vtb_cuda_state_create_paged): n_pages pages of page_size positions in kv_type
+    (synth.F32, F16 or BF16), with a sliding window and sinks if window > 0."""
+    n_pages: int
+    page_size: int = 64
+    kv_type: int = 0
+    window: int = 0
+    sinks: int = 0
+
+
 class CudaState:
     """KV cache + scratch for n_seqs sequences (vtb_cuda_state_create)."""
 
-    def __init__(self, model: CudaModel, n_seqs: int = 1, max_rows: int = 256):
+    def __init__(self, model: CudaModel, n_seqs: int = 1, max_rows: int = 256, paged: "PagedConfig | None" = None):
         self.model, self.lib, self.cfg = model, model.lib, model.cfg
         self.n_seqs = n_seqs
-        self.h = self.lib.vtb_cuda_state_create(model.h, n_seqs, max(max_rows, n_seqs))
-        if not self.h:
-            raise _lib.VtbError(-4, "vtb_cuda_state_create")
+        if paged is None:
+            self.h = self.lib.vtb_cuda_state_create(model.h, n_seqs, max(max_rows, n_seqs))
+            if not self.h:
+                raise _lib.VtbError(-4, "vtb_cuda_state_create")
+        else:
+            pc = _lib.PagedConfig(paged.page_size, paged.n_pages, paged.kv_type, paged.window, paged.sinks)
+            self.h = self.lib.vtb_cuda_state_create_paged(model.h, n_seqs, max(max_rows, n_seqs), C.byref(pc))
+            if not self.h:
+                raise _lib.VtbError(self.lib.vtb_cuda_last_status(), "vtb_cuda_state_create_paged")
 
     def close(self):
         if self.h:
@@ -337,6 +354,24 @@ class CudaState:
 
     def pos(self, seq: int = 0) -> int:
         return self.lib.vtb_cuda_state_pos(self.h, seq)
+
+    def fork(self, dst: int, src: int):
+        """Sequence dst becomes a copy of src (paged states: whole pages are shared)."""
+        _lib.check(self.lib.vtb_cuda_state_fork(self.h, dst, src), "vtb_cuda_state_fork")
+
+    def release(self, seq: int):
+        """Gives back a sequence's pages (paged states); its position becomes 0."""
+        _lib.check(self.lib.vtb_cuda_state_release(self.h, seq), "vtb_cuda_state_release")
+
+    def free_pages(self) -> int:
+        return self.lib.vtb_cuda_state_free_pages(self.h)
+
+    def compact(self) -> int:
+        """Moves the pages in use to the front of the pool; returns how many there are."""
+        n = self.lib.vtb_cuda_state_compact(self.h)
+        if n < 0:
+            _lib.check(n, "vtb_cuda_state_compact")
+        return n
 
     def tp_p2p(self) -> bool:
         """True when tensor-parallel all-reduces go over NVLink peer memory."""
