@@ -7,6 +7,7 @@ tensors are flat ``torch.uint8`` CUDA tensors of packed GGUF blocks.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import struct
 
 import torch
@@ -156,6 +157,7 @@ _KV = struct.Struct("@2P4i4qPq2i")
 _ROWS = struct.Struct("@2iq3P6q2Pq2P")
 _ATTN = struct.Struct("@2P4q3if2PN")
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 
 
 def _stream_of(dev: int) -> int:
@@ -172,28 +174,32 @@ def _on(dev: int, dtype: torch.dtype, **tensors) -> None:
 
 def _paged_kv(k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor | None):
     """The cache as the C ABI describes it; k, v [n_pages, n_kv_heads, page_size, head_dim]
-    (any order of strides, so a [page, slot, head, dim] cache goes in as .transpose(1, 2)).
-    Returns (descriptor, device index, dtype, shape, n_seqs)."""
+    (any order of strides, so a [page, slot, head, dim] cache goes in as .transpose(1, 2); an axis of
+    layers before them is left to the caller).  Returns (descriptor, device index, dtype, shape, n_seqs)."""
     dev, dt, st, shape = k.get_device(), k.dtype, k.stride(), k.shape
-    if dev < 0 or dev != torch.cuda.current_device():
+    if dev < 0 or dev != _current_device():
         raise ValueError("the cache must be on the current CUDA device")
-    if len(st) != 4 or st[3] != 1 or dt not in KV_TYPES:
+    code = KV_TYPES.get(dt)
+    if code is None or len(st) < 4 or st[-1] != 1:
         raise ValueError("the cache is [n_pages, n_kv_heads, page_size, head_dim], f32, f16 or bf16, dense in head_dim")
     if v.get_device() != dev or v.dtype is not dt or v.stride() != st or v.shape != shape:
         raise ValueError("k and v must agree in device, type, shape and strides")
-    n_pages, n_kv, page_size, hd = shape
-    if page_table is None:
-        table = (0, 0, 0, 0)
-    else:
-        _on(dev, torch.int32, page_table=page_table)
+    n_pages, n_kv, page_size, hd = shape[-4:]
+    ptr = ld = n = per = 0
+    if page_table is not None:
+        if page_table.get_device() != dev or page_table.dtype is not torch.int32:
+            _on(dev, torch.int32, page_table=page_table)
         if page_table.dim() != 2:
             raise ValueError("page_table is [n_seqs, pages per sequence]")
-        (n, per), (ld, one) = page_table.shape, page_table.stride()
+        n, per = page_table.shape
+        ld, one = page_table.stride()
         if one != 1 and per > 1:
             raise ValueError("page_table must be dense in its rows")
-        table = (page_table.data_ptr(), ld if n > 1 else max(ld, per), n, per)
-    kv = _KV.pack(k.data_ptr(), v.data_ptr(), KV_TYPES[dt], n_kv, hd, page_size, n_pages, st[0], st[1], st[2], *table)
-    return kv, dev, dt, shape, table[2]
+        if n <= 1 and ld < per:
+            ld = per
+        ptr = page_table.data_ptr()
+    kv = _KV.pack(k.data_ptr(), v.data_ptr(), code, n_kv, hd, page_size, n_pages, st[-4], st[-3], st[-2], ptr, ld, n, per)
+    return kv, dev, dt, shape, n
 
 
 def _rows(x: torch.Tensor, name: str, dev: int, dtype: torch.dtype, heads: int | None, hd: int):
@@ -224,7 +230,8 @@ def paged_append(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch
     pos[r] of sequence seq[r] (int32; a negative one skips the row), rotated by rope [positions, head_dim] if
     given; with q [rows, n_heads, head_dim] also returns the rotated queries in the cache's type (in q_out)."""
     kv, dev, dt, shape, _ = _paged_kv(k_pages, v_pages, page_table)
-    n_kv, hd, x = shape[1], shape[3], k.dtype
+    _, n_kv, _, hd = shape
+    x = k.dtype
     if x is not torch.float32 and x is not dt:
         raise ValueError("rows must be f32 or of the cache's type")
     ks = _rows(k, "k", dev, x, n_kv, hd)
@@ -260,23 +267,28 @@ def paged_append(k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch
     return q_out
 
 
+@functools.lru_cache(maxsize=None)
+def _workspace_bytes(dtype: torch.dtype, n_heads: int, n_kv_heads: int, head_dim: int, dev: int) -> int:
+    return lib.vtb_cuda_paged_attn_workspace_bytes(KV_TYPES[dtype], n_heads, n_kv_heads, head_dim)
+
+
 def paged_attention_workspace(dtype: torch.dtype, n_heads: int, n_kv_heads: int, head_dim: int,
                               device="cuda") -> torch.Tensor:
     """A workspace for the paged attention calls of one stream (calls that may overlap need one each)."""
-    n = lib.vtb_cuda_paged_attn_workspace_bytes(KV_TYPES[dtype], n_heads, n_kv_heads, head_dim)
+    n = _workspace_bytes(dtype, n_heads, n_kv_heads, head_dim, _current_device())
     return torch.empty(n, dtype=torch.uint8, device=device)
 
 
 def _attn(q, k_pages, dev, dt, shape, n_seqs, lens, scale, window, sinks, out, workspace):
-    n_kv, hd = shape[1], shape[3]
+    _, n_kv, _, hd = shape
     qs, heads = _rows(q, "q", dev, dt, None, hd), q.shape[1]
     if out is None:
-        out = torch.empty(q.shape, dtype=dt, device=k_pages.device)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(q.shape)
     os = _rows(out, "out", dev, dt, heads, hd)
     if out.shape[0] != q.shape[0]:
         raise ValueError("out must have q's shape")
     if workspace is None:
-        workspace = paged_attention_workspace(dt, heads, n_kv, hd, k_pages.device)
+        workspace = k_pages.new_empty(_workspace_bytes(dt, heads, n_kv, hd, dev), dtype=torch.uint8)
     elif workspace.get_device() != dev or workspace.dtype is not torch.uint8 or not workspace.is_contiguous():
         raise ValueError("workspace must be a contiguous uint8 tensor on the cache's device")
     a = _ATTN.pack(q.data_ptr(), out.data_ptr(), *qs, *os, heads, window, sinks, hd ** -0.5 if scale is None else scale,
@@ -316,17 +328,16 @@ def paged_copy(k_cache: torch.Tensor, v_cache: torch.Tensor, src: torch.Tensor, 
                page_table: torch.Tensor | None = None, page_map: torch.Tensor | None = None) -> None:
     """Copies page src[i] to page dst[i] (int32) in all layers of k_cache, v_cache [n_layers, n_pages, n_kv_heads,
     page_size, head_dim] (or one layer's 4-d pages); entries e >= 0 of page_table become page_map[e]."""
-    if k_cache.dim() == 4:
-        k_cache, v_cache = k_cache[None], v_cache[None]
-    if k_cache.dim() != 5 or v_cache.shape != k_cache.shape or v_cache.stride() != k_cache.stride() or not k_cache.shape[0]:
-        raise ValueError("the cache is [n_layers, n_pages, n_kv_heads, page_size, head_dim], k and v alike")
+    layers, step = (k_cache.shape[0], k_cache.stride(0)) if k_cache.dim() == 5 else (1, 0)
+    if k_cache.dim() not in (4, 5) or not layers:
+        raise ValueError("the cache is [n_layers, n_pages, n_kv_heads, page_size, head_dim], or one layer's four axes")
     if (page_table is None) != (page_map is None):
         raise ValueError("page_table and page_map go together")
-    kv, dev, _, shape, _ = _paged_kv(k_cache[0], v_cache[0], page_table)
+    kv, dev, _, shape, _ = _paged_kv(k_cache, v_cache, page_table)
     n = src.numel()
     moves = (_vec(src, "src", dev, n), _vec(dst, "dst", dev, n), n)
-    tables = (page_table.data_ptr(), _vec(page_map, "page_map", dev, shape[0])) if page_map is not None else (0, 0)
-    _lib.check(lib.vtb_cuda_paged_copy(kv, k_cache.shape[0], k_cache.stride(0), *moves, *tables, _stream_of(dev)),
+    tables = (page_table.data_ptr(), _vec(page_map, "page_map", dev, shape[-4])) if page_map is not None else (0, 0)
+    _lib.check(lib.vtb_cuda_paged_copy(kv, layers, step, *moves, *tables, _stream_of(dev)),
                "vtb_cuda_paged_copy")
 
 
