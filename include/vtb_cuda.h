@@ -219,7 +219,8 @@ int vtb_cuda_paged_append(const VtbCudaPagedKv *kv, const VtbCudaPagedRows *rows
  * multiple of n_kv_heads, 128 times it at most (query head h reads kv head h / (n_heads / n_kv_heads)).
  * lens[s] counts the cached positions of sequence s, the new ones included.  A
  * query at position p sees t <= p, with window > 0 only t > p - window or
- * t < sinks.  Softmax and sums are in f32.  A query that sees nothing gets zeros. */
+ * t < sinks.  Softmax and sums are in f32.  A query that sees nothing gets zeros; what a
+ * query does not see, infinities and NaN included, does not reach its output. */
 typedef struct VtbCudaPagedAttn {
   const void *q;
   void *out;

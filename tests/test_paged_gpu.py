@@ -242,6 +242,35 @@ def test_zero_scale_is_the_mean(dtype):
             assert torch.allclose(g[s].double().cpu(), mean, rtol=2 * P.EPS[dtype], atol=2 * P.EPS[dtype])
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page", [2, 16])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (70, 5)])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_prefill_hidden_infinities_and_nans(dtype, page, window, sinks, value):
+    """K and V of some tokens of the chunk are not finite: the queries that do not see them are as without them.
+    (Sequence 0: 210 new tokens on 40; 1: one new token, over a split.)"""
+    cache = P.Cache([250, 1300], 2, 64, page, dtype, 35)
+    at = [45, 100, 101, 233]
+    for t in at:
+        pg, slot = int(cache.table[0, t // page]), t % page
+        cache.k[pg, :, slot, 3] = value
+        cache.v[pg, 1, slot, 5] = value
+    g = torch.Generator().manual_seed(2)
+    q = torch.randn(211, 8, 64, generator=g).to(dtype).cuda()
+    got = ops.paged_attention_prefill(q, cache.k, cache.v, cache.table, cache.d_lens,
+                                      torch.tensor([0, 210, 211], dtype=torch.int32, device="cuda"), window=window, sinks=sinks)
+    ops.check_device_error()
+    pos = torch.arange(40, 250)
+    see = P.visible(pos, torch.tensor(at), window, sinks).any(1)
+    assert bool(see.any()) and not bool(see.all())
+    ref, a, b = P.attention(q[:210].double().cpu(), cache.k_rows[0].double(), cache.v_rows[0].double(), pos, 0.125, window, sinks)
+    tol = P.attention_tolerance(ref, a, b, 250, dtype, P_ROUNDED["prefill"])
+    clean = ~see
+    assert bool(((got[:210].double().cpu() - ref).abs() <= tol)[clean].all())
+    assert not bool(torch.isfinite(got[:210].float().cpu()[see][:, 4:]).all())  # kv head 1's queries that see them
+    check_rows(got[210:], cache, 1, q[210:], torch.tensor([1299]), 0.125, window, sinks, "prefill")
+
+
 def test_prefill_rows_before_the_first_position_give_zeros():
     """A chunk longer than the sequence's length: its first rows see nothing."""
     cache = P.Cache([10], 1, 64, 16, BF16, 27)

@@ -49,6 +49,7 @@ template <int HD> struct F32Prefill {
 struct F32Bars {
   uint64_t q_full, k_full, k_freed, v_full, v_freed, s_full, p_full, o_full;
   uint32_t tmem;
+  int by_rows;  // a V row that may be hidden from some query rows is infinite or NaN (attend_row)
 };
 
 template <int HD>
@@ -73,6 +74,7 @@ __global__ void __launch_bounds__(F_THREADS, 1) paged_prefill_f32_kernel(const _
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&bar.tmem)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   } else if (threadIdx.x == 0) {
+    bar.by_rows = 0;
     mbar_init(&bar.q_full, 4);
     mbar_init(&bar.k_full, 4);
     mbar_init(&bar.v_full, 4);
@@ -203,6 +205,7 @@ __global__ void __launch_bounds__(F_THREADS, 1) paged_prefill_f32_kernel(const _
           x[i] = *reinterpret_cast<const float*>(a.kv.v + off + d * 4);
         }
       };
+      bool odd = false;
       if (n > 0) fetch(0);
       for (int j = 0; j < n; ++j) {
         if (j) ok = warp_wait(&bar.v_freed, (j - 1) & 1);
@@ -213,10 +216,15 @@ __global__ void __launch_bounds__(F_THREADS, 1) paged_prefill_f32_kernel(const _
           const uint32_t at = sv + (pc >> 3) * (HD * 128) + d * 128 + (((pc & 7) ^ (d & 7)) << 4);
           uint32_t hi[4], lo[4];
 #pragma unroll
-          for (int c = 0; c < 4; ++c) split_tf32((j0 + j) * FN + p0 + i + c < sp.n ? x[i + c] : 0.f, hi[c], lo[c]);
+          for (int c = 0; c < 4; ++c) {
+            const float v = (j0 + j) * FN + p0 + i + c < sp.n ? x[i + c] : 0.f;
+            odd |= (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u;
+            split_tf32(v, hi[c], lo[c]);
+          }
           st4(at, hi);
           st4(at + C::KV, lo);
         }
+        if (__any_sync(0xffffffffu, odd) && lane == 0) bar.by_rows = 1;
         landed(&bar.v_full);
         if (j + 1 < n) fetch(j + 1);
       }
@@ -344,6 +352,18 @@ __global__ void __launch_bounds__(F_THREADS, 1) paged_prefill_f32_kernel(const _
     // ---------------- output: whole rows through shared memory ----------------
     if (ok) {
       float* part = a.part + (long long)blockIdx.x * C::SLOT;
+      if (n > 0 && *reinterpret_cast<volatile int*>(&bar.by_rows) && row) {
+        float acc[HD];
+        for (int i = 0; i < HD; ++i) acc[i] = 0.f;
+        m = -INFINITY;
+        l = 0.f;
+        const int t = a.token(r), head = kvh * a.group + r - t * a.group;
+        const float* q = static_cast<const float*>(a.q) + (rt.r0 + tok0 + t) * a.q_row + head * a.q_head;
+        for (int i = j0 * FN; i < min((j0 + n) * FN, sp.n); ++i)
+          attend_row<float, HD>(a, rt.s, kvh, q, rt.ctx + tok0 + t, sp.pos(i), sp.pos(i) + 1, m, l, acc);
+#pragma unroll
+        for (int i = 0; i < HD; ++i) o[i] = acc[i];
+      }
       const float inv = splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
       __syncwarp();
 #pragma unroll

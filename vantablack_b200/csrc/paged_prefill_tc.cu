@@ -18,11 +18,12 @@
 //
 // Warps 0-3: softmax of A; 4-7: of B; 8: issues the MMAs; 10: brings Q, K and V
 // by TMA, K and V into two stages each, one box per page and 64 values (4-d map
-// over the page pool); 11: puts zeros in place of V rows at positions that no
-// query row sees (behind the last position, before the window), so that what lies
-// in the rest of a page never meets P = 0.  Pages of fewer than 8 positions, whose
-// boxes would break the swizzle, are gathered row by row with cp.async by warps
-// 10 and 11.  Warp 9 only completes the warpgroup.
+// over the page pool); 9 and 11: in tiles at an edge (the last positions, the
+// window's start) put zeros in place of V rows at positions that no query row
+// sees, so that what lies in the rest of a page never meets P = 0, and look for
+// infinities and NaN in the others (attend_row).  Pages of fewer than 8 positions,
+// whose boxes would break the swizzle, are gathered row by row with cp.async by
+// warps 9 to 11.
 //
 // The scale is taken positive (a negative one negates Q in the first product),
 // so the maximum of S is the maximum of the scaled scores.
@@ -104,6 +105,33 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
+// Rows one by one, for tiles in which a V row that only part of the query rows
+// see holds an infinity or a NaN: 0 * inf in the tile products would carry it to
+// the rows that do not see it.  Adds the positions [t0, t1) that a query at
+// position p sees to (m, l, acc), in f32.
+template <typename T, int HD>
+__device__ __noinline__ void attend_row(const AttnArgs& a, int s, int kvh, const T* q, int p, int t0, int t1, float& m, float& l,
+                                        float* acc) {
+  const int32_t* table = a.kv.table + s * a.kv.table_stride;
+  for (int t = t0; t < t1 && t <= p; ++t) {
+    if (a.window && t <= p - a.window && t >= a.sinks) continue;
+    const long long off = page_row(a.kv, __ldg(table + (t >> a.kv.page_shift)), t) + kvh * a.kv.head_stride;
+    const T *k = reinterpret_cast<const T*>(a.kv.k + off), *v = reinterpret_cast<const T*>(a.kv.v + off);
+    float x = 0.f;
+    for (int d = 0; d < HD; ++d) x = fmaf(to_f(q[d]), to_f(k[d]), x);
+    x *= a.negate ? -a.scale2 : a.scale2;
+    const float mn = fmaxf(m, x), b = mn == -INFINITY ? 0.f : mn, f = exp2f(m - b), e = exp2f(x - b);
+    m = mn;
+    l = l * f + e;
+    for (int d = 0; d < HD; ++d) acc[d] = acc[d] * f + e * to_f(v[d]);
+  }
+}
+// Whether one of the 16-bit values in w is infinite or NaN, in bits 15 and 31 of the result.
+template <typename T> __device__ __forceinline__ uint32_t nonfinite2(uint32_t w) {
+  constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+  return (w & e) + (std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u);
+}
+
 constexpr int TQ = 128, TN = 128, TC_THREADS = 384;
 // Registers per thread after the split: softmax warps, MMA and gather warps.
 // setmaxnreg draws on what the CTA was launched with, so the sum of the shares
@@ -120,6 +148,7 @@ template <int HD> struct TcPrefill {
 struct TcBars {
   uint64_t q_full, q_freed, k_full[2], k_freed[2], v_full[2], v_freed[2], v_raw[2], s_full[2], p_full[2], o_full[2], done;
   uint32_t tmem;
+  int rows_of[4];  // [i & 3] = i + 1: the CTA's i-th item is to be done row by row
 };
 
 // One piece of work: two row tiles of a kv head over one split of the positions they see.
@@ -176,12 +205,13 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&bar.tmem)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   } else if (threadIdx.x == 0) {
+    for (int i = 0; i < 4; ++i) bar.rows_of[i] = 0;
     mbar_init(&bar.q_full, 1);
     mbar_init(&bar.q_freed, 1);
     mbar_init(&bar.done, 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar.k_full[i], 2);  // warps 10 and 11
-      mbar_init(&bar.v_full[i], 2);
+      mbar_init(&bar.k_full[i], box ? 2 : 3);  // warp 10 twice, or warps 9 to 11
+      mbar_init(&bar.v_full[i], 3);
       mbar_init(&bar.k_freed[i], 1);
       mbar_init(&bar.v_freed[i], 1);
       mbar_init(&bar.v_raw[i], 1);
@@ -286,7 +316,7 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
       }
       signal(&bar.done);
       warp_wait(&bar.done, 0);  // nothing is in flight when the columns are given back
-    } else if (warp >= 10) {
+    } else {
       // ---------------- Q rows, K / V tiles ----------------
       const int pc = lane % PIECES, sub = lane / PIECES;
       auto landed = [&](uint64_t* full) {  // this warp's writes are in shared memory
@@ -294,7 +324,7 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
         __syncwarp();
         if (lane == 0) mbar_arrive(full);
       };
-      int kt = 0, nq = 0;
+      int kt = 0, nq = 0, ni = -1;
       unsigned edges = 0;  // phase of v_raw[i] in bit i
       for (int k = 0; ok; ++k) {
         const int i = tc_deal(k);
@@ -302,7 +332,9 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
         if (!tc_item(a, i, items, splits, it)) continue;
         const RowTile& rt = it.rt;
         const int32_t* table = a.kv.table + rt.s * a.kv.table_stride;
-        const int n = it.tiles(), p1 = it.p1, w0 = it.w0;
+        const int n = it.tiles(), p1 = it.p1, w0 = it.w0, first = rt.ctx + rt.f0 / a.group;
+        ++ni;
+        uint32_t odd = 0;  // nonfinite2 of V rows that only part of the item's rows see
         if (warp == 10) {  // Q: both tiles, a box of (64 values, group, tokens of a tile) each
           if (nq) ok = warp_wait(&bar.q_freed, (nq - 1) & 1);
           if (!ok) break;
@@ -339,7 +371,7 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
           src += it.kvh * a.kv.head_stride + pc * 16;
           const uint32_t d = dst + (pc >> 3) * C::ATOM;
 #pragma unroll 4
-          for (int r = (warp - 10) * RPW + sub; r < TN; r += 2 * RPW) {
+          for (int r = (warp - 9) * RPW + sub; r < TN; r += 3 * RPW) {
             const int pos = t0 + r;
             const bool live = pos <= p1 && (pos >= w0 || pos < a.sinks);
             const long long off = live ? page_row(a.kv, __ldg(table + (pos >> a.kv.page_shift)), pos) : 0;
@@ -347,10 +379,18 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
           }
           cpa_commit();
         };
+        auto look = [&](uint32_t at) {
+          uint32_t x[4];
+          asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
+          odd |= nonfinite2<T>(x[0]) | nonfinite2<T>(x[1]) | nonfinite2<T>(x[2]) | nonfinite2<T>(x[3]);
+        };
+        auto report = [&]() {
+          if (__any_sync(0xffffffffu, odd & 0x80008000u) && lane == 0) bar.rows_of[ni & 3] = ni + 1;
+        };
         for (int j = 0; j < n; ++j, ++kt) {
           const int t0 = it.pos(j), slot = kt & 1;
           const uint32_t ak = sk + slot * C::TILE, av = sv + slot * C::TILE;
-          // (with boxes warp 11 only follows the edge tiles, by v_raw)
+          // (with boxes warps 9 and 11 only follow the edge tiles, by v_raw)
           const bool fills = warp == 10 || !box;
           if (fills && kt >= 2) ok = warp_wait(&bar.k_freed[slot], ((kt >> 1) - 1) & 1);
           if (!ok) break;
@@ -367,9 +407,11 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
             cpa_wait<1>();
             landed(&bar.k_full[slot]);
             cpa_wait<0>();
+            for (int r = (warp - 9) * RPW + sub; r < TN; r += 3 * RPW) look(av + (pc >> 3) * C::ATOM + r * 128 + (((pc & 7) ^ (r & 7)) << 4));
+            report();
             landed(&bar.v_full[slot]);
-          } else if (t0 + TN > p1 + 1 || (t0 < w0 && t0 + TN > a.sinks)) {
-            // an edge tile: zeros in place of the V rows that no query row sees
+          } else if (t0 + TN > first + 1 || (a.window && t0 < p1 + 1 - a.window)) {
+            // an edge tile: zeros in place of the V rows that no query row sees, and a look at the others
             if (warp == 10) {
               if (lane == 0) mbar_arrive(&bar.v_full[slot]);
               boxes(&map_v, av, t0, &bar.v_raw[slot]);
@@ -377,16 +419,21 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
               ok = warp_wait(&bar.v_raw[slot], edges >> slot & 1);
               if (!ok) break;
               edges ^= 1u << slot;
-              for (int r = sub; r < TN; r += RPW) {
-                const int pos = t0 + r;
-                if (pos > p1 || (pos < w0 && pos >= a.sinks))
-                  *reinterpret_cast<uint4*>(smem + (4 + slot) * C::TILE + (pc >> 3) * C::ATOM + r * 128 + ((pc & 7) << 4)) =
-                      make_uint4(0, 0, 0, 0);
-              }
+              const int r0 = (warp == 11 ? TN / 2 : 0) + sub;
+              if (t0 + TN > p1 + 1 || (t0 < w0 && t0 + TN > a.sinks))
+                for (int r = r0; r < r0 + TN / 2; r += RPW) {
+                  const int pos = t0 + r;
+                  if (pos > p1 || (pos < w0 && pos >= a.sinks))
+                    *reinterpret_cast<uint4*>(smem + (4 + slot) * C::TILE + (pc >> 3) * C::ATOM + r * 128 + ((pc & 7) << 4)) =
+                        make_uint4(0, 0, 0, 0);
+                }
+#pragma unroll 8
+              for (int i = 0; i < TN / 2; i += RPW) look(av + (pc >> 3) * C::ATOM + (r0 + i) * 128 + ((pc & 7) << 4));
+              report();
               landed(&bar.v_full[slot]);
             }
           } else if (warp == 10) {
-            if (lane == 0) mbar_arrive(&bar.v_full[slot]);
+            if (lane < 2) mbar_arrive(&bar.v_full[slot]);
             boxes(&map_v, av, t0, &bar.v_full[slot]);
           }
         }
@@ -399,11 +446,12 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
     const int w = warp >> 2, r = threadIdx.x & 127;
     const uint32_t ts = w * TN + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t to = 256 + w * HD + ((uint32_t)((warp & 3) * 32) << 16);
-    int ns = 0, no = 0;  // S and O tiles so far
+    int ns = 0, no = 0, ni = -1;  // S and O tiles, items so far
     for (int k = 0; ok; ++k) {
       const int item = tc_deal(k);
       if (item >= items) break;
       if (!tc_item(a, item, items, splits, it)) continue;
+      ++ni;
       const RowTile& rt = it.rt;
       const int f = rt.f0 + w * a.tile + r;
       const bool row = r < a.tile && f < it.nflat;
@@ -490,6 +538,31 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
       if (!ok) break;
       tc_fence_after();
       float* part = a.part + (long long)item * C::SLOT;
+      if (m_tiles > 0 && *reinterpret_cast<volatile int*>(&bar.rows_of[ni & 3]) == ni + 1) {
+        if (row) {
+          float acc[HD];
+          for (int d = 0; d < HD; ++d) acc[d] = 0.f;
+          m = -INFINITY;
+          l = 0.f;
+          const int head = it.kvh * a.group + r - a.token(r) * a.group;
+          const long long tok = rt.r0 + tok0 + a.token(r);
+          for (int j = 0; j < m_tiles; ++j)
+            attend_row<T, HD>(a, rt.s, it.kvh, static_cast<const T*>(a.q) + tok * a.q_row + head * a.q_head, vc - 1, it.pos(j), it.pos(j) + TN,
+                              m, l, acc);
+          T* out = static_cast<T*>(a.out) + tok * a.o_row + head * a.o_head;
+          for (int d = 0; d < HD; ++d) {
+            if (splits == 1) out[d] = from_f<T>(l == 0.f ? 0.f : acc[d] / l);
+            else part[4 * TQ + (long long)(w * TQ + r) * HD + d] = acc[d];
+          }
+          if (splits > 1) {
+            part[w * TQ + r] = m;
+            part[2 * TQ + w * TQ + r] = l;
+          }
+        }
+        __syncwarp();
+        tc_fence_before();
+        continue;
+      }
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const uint32_t stage = sq + 6 * C::TILE + warp * 32 * 128;  // 64 values of this warp's 32 rows
       // Rows go out whole, 8 lanes to 128 bytes: this lane's rows are lane / 8 + 4 i.
