@@ -1,7 +1,7 @@
 // paged_prefill_tc.cu -- chunk attention over the paged cache on the 5th-
 // generation tensor cores, for f16 and bf16 caches.
 //
-// One CTA per SM walks a list of items.  An item is two tiles A and B of up to
+// One CTA per SM runs at a time and takes items one after the other.  An item is two tiles A and B of up to
 // 128 query rows of one kv head (rows = (token, head of the group) pairs in token
 // order, whole tokens to a tile), and the positions they see in tiles of 128.
 // Per tile of positions:
@@ -146,6 +146,8 @@ template <int HD> struct TcPrefill {
 };
 
 struct TcBars {
+  uint4 answer[2];  // to requests for items
+  uint64_t next_full[2], next_read[2];
   uint64_t q_full, q_freed, k_full[2], k_freed[2], v_full[2], v_freed[2], v_raw[2], s_full[2], p_full[2], o_full[2], done;
   uint32_t tmem;
   int rows_of[4];  // [i & 3] = i + 1: the CTA's i-th item is to be done row by row
@@ -182,10 +184,26 @@ __device__ __forceinline__ bool tc_item(const AttnArgs& a, int i, int items, int
   t.nb = rt.f0 + a.tile < t.nflat ? j1 - t.j0 : 0;
   return true;
 }
-// A CTA's k-th item: the list is dealt in rows of gridDim.x, every other row
-// backwards, so that CTAs with a long first item get a short second one.
-__device__ __forceinline__ int tc_deal(int k) {
-  return k * (int)gridDim.x + (int)((k & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+// Work is taken as it is needed: the grid has a CTA per item, and a CTA that runs
+// takes over the item of one that has not started (cluster launch control), so
+// ragged batches even out without a counter in memory.  The request for the next
+// item is made with the loads of this one's last tile: early enough for its first
+// tiles to follow without a gap, late enough for long items to be nearly done.
+__device__ __forceinline__ void request_item(uint32_t answer, uint64_t* bar) {
+  mbar_expect_tx(bar, 16);
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+               ::"r"(answer), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ int requested_item(uint32_t answer) {  // -1: none is left
+  int got, x;
+  asm volatile(
+      "{\n .reg .b128 h;\n .reg .pred p;\n .reg .b32 y, z, w;\n"
+      " ld.shared.b128 h, [%2];\n"
+      " clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, h;\n"
+      " selp.s32 %0, 1, 0, p;\n mov.b32 %1, 0;\n"
+      " @p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, y, z, w}, h;\n}\n"
+      : "=r"(got), "=r"(x) : "r"(answer) : "memory");
+  return got ? x : -1;
 }
 
 template <typename T, int HD>
@@ -218,6 +236,8 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
       mbar_init(&bar.s_full[i], 1);
       mbar_init(&bar.p_full[i], 4);  // the tile's four warps
       mbar_init(&bar.o_full[i], 1);
+      mbar_init(&bar.next_full[i], 1);
+      mbar_init(&bar.next_read[i], TC_THREADS / 32);
     }
     fence_mbar_init();
   } else if (warp == 10 && lane == 0) {
@@ -235,6 +255,21 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
   const uint32_t tmem = bar.tmem;
   bool ok = true;  // one answer per warp; a wait that gave up ends the warp's work
   TcItem it;
+  // The CTA's items: number 0 is its own, number q >= 1 the answer to request q (slot q & 1).
+  auto phase_of = [](int q) { return (((q + 1) >> 1) - 1) & 1; };
+  auto request = [&](int q) {
+    if (q >= 3) ok = ok && warp_wait(&bar.next_read[q & 1], phase_of(q - 2));  // every warp has read the slot's last answer
+    if (ok && lane == 0) request_item(smem_u32(&bar.answer[q & 1]), &bar.next_full[q & 1]);
+  };
+  auto next_item = [&](int q) -> int {
+    ok = ok && warp_wait(&bar.next_full[q & 1], phase_of(q));
+    if (!ok) return -1;
+    const int i = requested_item(smem_u32(&bar.answer[q & 1]));
+    fence_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bar.next_read[q & 1]);
+    return i;
+  };
 
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS_OTHER));
@@ -279,9 +314,7 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
         tc_fence_after();
       };
       int kt = 0, np[2] = {0, 0}, nq = 0;  // position tiles, P tiles of A and B, items so far
-      for (int k = 0; ok; ++k) {
-        const int i = tc_deal(k);
-        if (i >= items) break;
+      for (int k = 1, i = blockIdx.x; i >= 0; i = next_item(k++)) {
         if (!tc_item(a, i, items, splits, it)) continue;
         const int n = it.tiles();
         wait(&bar.q_full, nq++);
@@ -326,10 +359,10 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
       };
       int kt = 0, nq = 0, ni = -1;
       unsigned edges = 0;  // phase of v_raw[i] in bit i
-      for (int k = 0; ok; ++k) {
-        const int i = tc_deal(k);
-        if (i >= items) break;
-        if (!tc_item(a, i, items, splits, it)) continue;
+      for (int k = 1, i = blockIdx.x; i >= 0; i = next_item(k++)) {
+        const bool any = tc_item(a, i, items, splits, it);
+        if (warp == 10 && (!any || it.tiles() == 0)) request(k);
+        if (!any) continue;
         const RowTile& rt = it.rt;
         const int32_t* table = a.kv.table + rt.s * a.kv.table_stride;
         const int n = it.tiles(), p1 = it.p1, w0 = it.w0, first = rt.ctx + rt.f0 / a.group;
@@ -388,6 +421,7 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
           if (__any_sync(0xffffffffu, odd & 0x80008000u) && lane == 0) bar.rows_of[ni & 3] = ni + 1;
         };
         for (int j = 0; j < n; ++j, ++kt) {
+          if (warp == 10 && j + 1 == n) request(k);
           const int t0 = it.pos(j), slot = kt & 1;
           const uint32_t ak = sk + slot * C::TILE, av = sv + slot * C::TILE;
           // (with boxes warps 9 and 11 only follow the edge tiles, by v_raw)
@@ -447,9 +481,7 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
     const uint32_t ts = w * TN + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t to = 256 + w * HD + ((uint32_t)((warp & 3) * 32) << 16);
     int ns = 0, no = 0, ni = -1;  // S and O tiles, items so far
-    for (int k = 0; ok; ++k) {
-      const int item = tc_deal(k);
-      if (item >= items) break;
+    for (int k = 1, item = blockIdx.x; item >= 0; item = next_item(k++)) {
       if (!tc_item(a, item, items, splits, it)) continue;
       ++ni;
       const RowTile& rt = it.rt;
@@ -748,8 +780,7 @@ static cudaError_t launch_prefill_tc_t(AttnArgs a, cudaStream_t st) {
   const int box = slots >= 8 && page_map(&map_k, a.kv, a.kv.k, std::is_same<T, __half>::value, HD, a.n_kv, fit) &&
                           page_map(&map_v, a.kv, a.kv.v, std::is_same<T, __half>::value, HD, a.n_kv, fit) ? fit : 0;
   const long long items = units * splits;
-  const unsigned grid = (unsigned)(items < sm_count(dev) ? items : sm_count(dev));
-  paged_prefill_tc_kernel<T, HD><<<grid, TC_THREADS, C::SMEM, st>>>(a, map_k, map_v, map_q, (int)items, splits, box);
+  paged_prefill_tc_kernel<T, HD><<<(unsigned)items, TC_THREADS, C::SMEM, st>>>(a, map_k, map_v, map_q, (int)items, splits, box);
   if ((e = cudaGetLastError()) || splits == 1) return e;
   return launch_dependent(paged_prefill_join_kernel<T, HD, 2>, dim3((unsigned)(units * 16)), dim3(256), 0, st, a, splits);
 }
