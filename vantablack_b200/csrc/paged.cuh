@@ -144,12 +144,12 @@ template <typename T, int HD, int NT, bool F32 = Elem<T>::f32> struct Step;
 // exact to 2^-17 (bf16): the output then carries its own rounding only.
 template <typename T, int HD, int NT> struct Step<T, HD, NT, false> {
   static constexpr bool F = false;
-  static constexpr int PIECES = HD / 8, KROW = HD * 2, VROW = HD * 2;  // bytes per staged row
+  static constexpr int PIECES = HD / 8, ROW = HD * 2;  // 16-byte pieces and bytes of a staged row
   static constexpr int QREGS = HD / 8;
   uint32_t q[NT][QREGS];
 
-  static __device__ __forceinline__ uint32_t k_off(int r, int piece) { return r * KROW + ((piece ^ (r & 7)) << 4); }
-  static __device__ __forceinline__ uint32_t v_off(int r, int piece) { return r * VROW + ((piece ^ (r & 7)) << 4); }
+  static __device__ __forceinline__ uint32_t k_off(int r, int piece) { return r * ROW + ((piece ^ (r & 7)) << 4); }
+  static __device__ __forceinline__ uint32_t v_off(int r, int piece) { return r * ROW + ((piece ^ (r & 7)) << 4); }
   // Vector 8 nt + g's values, read from `p` (null: a vector of zeros).
   __device__ __forceinline__ void load_q(int nt, const T* p, int t) {
 #pragma unroll
@@ -212,16 +212,17 @@ template <typename T, int HD, int NT> struct Step<T, HD, NT, false> {
 // group.  The order of the head dimensions inside a product is free as long as
 // both operands share it, so a lane reads whole 16-byte pieces: score step
 // (jj, cc) holds dimensions 4 (t + 4 jj) + 2 cc + {0, 1} of lane t, output tile
-// (jj, cc) dimensions 4 (g + 8 jj) + 2 cc + {0, 1} of lane g.  Row pitches of
-// 64 (K) and 16 bytes (V) over a multiple of 128 keep these reads conflict-free.
+// (jj, cc) dimensions 4 (g + 8 jj) + 2 cc + {0, 1} of lane g.  The eight lanes of a
+// 128-byte phase read 4 pieces of two rows of K, 2 pieces of four rows of V: the
+// pieces are swizzled by the row so that these fall into different banks.
 template <int HD, int NT> struct Step<float, HD, NT, true> {
   static constexpr bool F = true;
-  static constexpr int PIECES = HD / 4, KROW = HD * 4 + 64, VROW = HD * 4 + 16;
+  static constexpr int PIECES = HD / 4, ROW = HD * 4;
   static constexpr int QREGS = HD / 4;
   float q[NT][QREGS];
 
-  static __device__ __forceinline__ uint32_t k_off(int r, int piece) { return r * KROW + (piece << 4); }
-  static __device__ __forceinline__ uint32_t v_off(int r, int piece) { return r * VROW + (piece << 4); }
+  static __device__ __forceinline__ uint32_t k_off(int r, int piece) { return r * ROW + ((piece ^ ((r & 1) << 2)) << 4); }
+  static __device__ __forceinline__ uint32_t v_off(int r, int piece) { return r * ROW + ((piece ^ (r & 6)) << 4); }
   __device__ __forceinline__ void load_q(int nt, const float* p, int t) {
 #pragma unroll
     for (int jj = 0; jj < HD / 16; ++jj) {

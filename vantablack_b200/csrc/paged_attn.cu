@@ -55,9 +55,12 @@ __device__ __forceinline__ Span span_of(int p0, int p1, int window, int sinks) {
 
 template <typename T, int HD, int NT> struct DecodeCfg {
   using S = Step<T, HD, NT>;
-  static constexpr int WARPS = S::F ? (HD == 128 ? 6 : 8) : HD == 64 ? 8 : 4, TILE = 16 * WARPS;
-  static constexpr int STAGE = 16 * (S::KROW + S::VROW);  // bytes: one warp's K and V rows
-  static constexpr int STAGES = S::F ? 2 : 3;
+  // A warp's ring holds the K and V rows of 16 positions, STAGES times; for f32 at 128 values, where
+  // eight warps have no room for two stages, K and V take turns in three halves (8 warps at 5.5 TB/s,
+  // 6 with two whole stages at 5.0; in halves the smaller rows lose 5 to 10%).
+  static constexpr int WARPS = S::F || HD == 64 ? 8 : 4, TILE = 16 * WARPS;
+  static constexpr bool HALVES = S::F && HD == 128;
+  static constexpr int STAGES = S::F && HD == 64 ? 2 : 3, ROWS = 16 * S::ROW, STAGE = HALVES ? ROWS : 2 * ROWS;
   static constexpr int RED = WARPS * 4 * (HD + 4) * 4;  // the warps' o of 4 query vectors
   static constexpr int SMEM = WARPS * STAGES * STAGE + RED + WARPS * 8 * 2 * 4;
   static constexpr int SLOT = NT * 8 * (HD + 2);  // floats of one partial result
@@ -161,8 +164,8 @@ paged_decode_kernel(const __grid_constant__ AttnArgs a, int hgroups) {
   const int n = (int)(w1 - w0);
 
   const uint32_t ring = smem_u32(smem) + warp * C::STAGES * C::STAGE;
-  // The row this lane looks up for the next tile to load (rows lane & 15), and its page:
-  // the table is read one tile ahead of the copies that need it.
+  // The row this lane looks up for the next tile to load (rows lane & 15): its page is
+  // read one tile ahead of the copies that need it.
   int row_pos = -1, row_page = 0;
   auto look = [&]() {
     const int i = ld.t * C::TILE + warp * 16 + (lane & 15);
@@ -172,29 +175,51 @@ paged_decode_kernel(const __grid_constant__ AttnArgs a, int hgroups) {
       row_page = a.kv.table[ld.s * a.kv.table_stride + (row_pos >> a.kv.page_shift)];
     }
   };
-  auto load = [&](int stage) {
-    const long long off = row_pos < 0 ? -1 : page_row(a.kv, row_page, row_pos) + (ld.u / hgroups) * a.kv.head_stride;
-    const uint32_t kd = ring + stage * C::STAGE, vd = kd + 16 * S::KROW;
-    constexpr int RPI = 32 / S::PIECES > 0 ? 32 / S::PIECES : 1;  // rows per round of 32 lanes
+  // Stages go out in order: a tile's K and V, or its K, for which the rows are found, and then its V.
+  int out_tile = 0, out_slot = 0;
+  bool out_v = false;
+  long long off = -1;
+  auto copy = [&](uint32_t dst, const char* base, bool v) {
+    constexpr int RPI = 32 / S::PIECES;  // rows per round of 32 lanes
 #pragma unroll
     for (int r0 = 0; r0 < 16; r0 += RPI) {
       const int r = r0 + lane / S::PIECES, pc = lane % S::PIECES;
-      const long long o = __shfl_sync(0xffffffffu, off, r);
-      const long long src = (o < 0 ? 0 : o) + pc * 16;
-      cpa16(kd + S::k_off(r, pc), a.kv.k + src, o >= 0);
-      cpa16(vd + S::v_off(r, pc), a.kv.v + src, o >= 0);
+      const long long o = __shfl_sync(0xffffffffu, off, r), src = (o < 0 ? 0 : o) + pc * 16;
+      if (C::HALVES) {
+        cpa16(dst + (v ? S::v_off(r, pc) : S::k_off(r, pc)), base + src, o >= 0);
+      } else {
+        cpa16(dst + S::k_off(r, pc), a.kv.k + src, o >= 0);
+        cpa16(dst + C::ROWS + S::v_off(r, pc), a.kv.v + src, o >= 0);
+      }
     }
   };
-  look();
-#pragma unroll
-  for (int i = 0; i < C::STAGES - 1; ++i) {
-    if (i < n) {
-      load(i);
-      ld.next(a, units);
-      if (i + 1 < n) look();
+  auto load = [&]() {
+    if (out_tile < n) {
+      const uint32_t dst = ring + out_slot * C::STAGE;
+      if (!C::HALVES || !out_v) {
+        off = row_pos < 0 ? -1 : page_row(a.kv, row_page, row_pos) + (ld.u / hgroups) * a.kv.head_stride;
+        ld.next(a, units);
+        if (out_tile + 1 < n) look();
+      }
+      copy(dst, out_v ? a.kv.v : a.kv.k, out_v);
+      out_tile += !C::HALVES || out_v;
+      out_v = !out_v;
+      out_slot = out_slot + 1 == C::STAGES ? 0 : out_slot + 1;
     }
     cpa_commit();
-  }
+  };
+  look();
+#pragma unroll 1
+  for (int i = 0; i < C::STAGES - 1; ++i) load();
+  int slot_now = 0;
+  auto arrived = [&]() -> uint32_t {  // the next stage, whole; the one before it makes room for another
+    cpa_wait<C::STAGES - 2>();
+    __syncwarp();
+    load();
+    const uint32_t at = ring + slot_now * C::STAGE;
+    slot_now = slot_now + 1 == C::STAGES ? 0 : slot_now + 1;
+    return at;
+  };
 
   S st;
   auto queries = [&](int s, int u) {  // the query vectors of unit u
@@ -220,19 +245,13 @@ paged_decode_kernel(const __grid_constant__ AttnArgs a, int hgroups) {
         for (int j = 0; j < HD / 16; ++j) o[nt][j][0] = o[nt][j][1] = o[nt][j][2] = o[nt][j][3] = 0.f;
       }
     }
-    cpa_wait<C::STAGES - 2>();
-    __syncwarp();
-    if (i + C::STAGES - 1 < n) {
-      load((i + C::STAGES - 1) % C::STAGES);
-      ld.next(a, units);
-      if (i + C::STAGES < n) look();
-    }
-    cpa_commit();
     const int base = cur.t * C::TILE + warp * 16;
-    if (base < cur.sp.n) {
-      const uint32_t kb = ring + (i % C::STAGES) * C::STAGE;
-      float s[NT][4];
-      st.scores(kb, lane, s);
+    const bool any = base < cur.sp.n;  // (the same for the whole warp)
+    float s[NT][4];
+    const uint32_t kb = arrived();
+    if (any) st.scores(kb, lane, s);
+    const uint32_t vb = C::HALVES ? arrived() : kb + C::ROWS;
+    if (any) {
       const bool in0 = base + g < cur.sp.n, in1 = base + g + 8 < cur.sp.n;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -243,7 +262,7 @@ paged_decode_kernel(const __grid_constant__ AttnArgs a, int hgroups) {
       }
       float f[NT][2];
       const bool moved = softmax_step<NT>(s, m, l, f);
-      st.pv(kb + 16 * S::KROW, lane, s, f, moved, o);
+      st.pv(vb, lane, s, f, moved, o);
     }
     if (cur.t + 1 < cur.nt && i + 1 < n) {
       ++cur.t;
