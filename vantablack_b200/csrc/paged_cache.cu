@@ -53,61 +53,58 @@ __device__ __forceinline__ void store_vec(T* p, const float (&x)[N]) {
   }
 }
 
-// HBM bound (each value read and written once).  The rotation is the forward
-// loop's: products and their difference rounded separately in f32, then one
-// rounding to the cache's type.
+// HBM bound (each value read and written once).  CTA (row, part) has 256 vectors of
+// a row, one per thread, so nothing is divided; its threads read the row's page
+// through the same cache lines.  The rotation is the forward loop's: products and
+// their difference rounded separately in f32, then one rounding to the cache's
+// type.
 template <typename X, typename T>
 __global__ void __launch_bounds__(256) paged_append_kernel(const __grid_constant__ AppendArgs a) {
   constexpr int N = 16 / sizeof(T);
-  const int per_head = a.hd / N, nq = a.q ? a.n_heads : 0, per_row = (nq + 2 * a.n_kv) * per_head;
-  const long long items = a.rows * per_row;
-  for (long long it = blockIdx.x * 256ll + threadIdx.x; it < items; it += gridDim.x * 256ll) {
-    const long long row = it / per_row;
-    const int rest = (int)(it - row * per_row), head = rest / per_head, d = (rest - head * per_head) * N;
-    const int pos = a.pos[row], seq = a.seq[row];
-    if (pos < 0 || seq < 0) continue;  // a padding row
-    if (seq >= a.kv.n_seqs || pos >= (long long)a.kv.pages_per_seq << a.kv.page_shift || (a.rope && pos >= a.n_rope)) {
-      flag_error(DEV_ERR_BAD_ARG);
-      continue;
-    }
-    const bool is_q = head < nq, is_v = head >= nq + a.n_kv;
-    const int h = is_q ? head : is_v ? head - nq - a.n_kv : head - nq;
-    T* dst;
-    if (is_q) {
-      dst = static_cast<T*>(a.q_out) + (row * a.n_heads + h) * a.hd + d;
-    } else {
-      const int page = a.kv.table[seq * a.kv.table_stride + (pos >> a.kv.page_shift)];
-      if ((unsigned)page >= (unsigned)a.kv.n_pages) {
-        flag_error(DEV_ERR_BAD_ARG);
-        continue;
-      }
-      const long long off = page_row(a.kv, page, pos) + h * a.kv.head_stride;
-      dst = reinterpret_cast<T*>(const_cast<char*>(is_v ? a.kv.v : a.kv.k) + off) + d;
-    }
-    const X* src = is_q   ? static_cast<const X*>(a.q) + row * a.q_row + h * a.q_head
-                   : is_v ? static_cast<const X*>(a.v) + row * a.v_row + h * a.v_head
-                          : static_cast<const X*>(a.k) + row * a.k_row + h * a.k_head;
-    float x[N];
-    load_vec<X, T>(src + d, x);
-    if (a.rope && !is_v) {
-      float cs[N];
-      load_vec<float, float>(a.rope + (long long)pos * a.hd + d, cs);
-#pragma unroll
-      for (int i = 0; i < N; i += 2) {
-        const float x0 = x[i], x1 = x[i + 1], c = cs[i], s = cs[i + 1];
-        x[i] = __fsub_rn(__fmul_rn(x0, c), __fmul_rn(x1, s));
-        x[i + 1] = __fadd_rn(__fmul_rn(x0, s), __fmul_rn(x1, c));
-      }
-    }
-    store_vec(dst, x);
+  const int shift = a.hd * (int)sizeof(T) == 512 ? 5 : a.hd * (int)sizeof(T) == 256 ? 4 : 3;  // log2 of vectors per head
+  const int nq = a.q ? a.n_heads : 0, i = blockIdx.y * 256 + threadIdx.x, head = i >> shift, d = (i & ((1 << shift) - 1)) * N;
+  if (head >= nq + 2 * a.n_kv) return;
+  const long long row = blockIdx.x;
+  const bool is_q = head < nq, is_v = head >= nq + a.n_kv;
+  const X* src = is_q   ? static_cast<const X*>(a.q) + row * a.q_row + head * a.q_head
+                 : is_v ? static_cast<const X*>(a.v) + row * a.v_row + (head - nq - a.n_kv) * a.v_head
+                        : static_cast<const X*>(a.k) + row * a.k_row + (head - nq) * a.k_head;
+  float x[N];
+  load_vec<X, T>(src + d, x);
+  const int pos = a.pos[row], seq = a.seq[row];
+  if (pos < 0 || seq < 0) return;  // a padding row
+  if (seq >= a.kv.n_seqs || pos >= (long long)a.kv.pages_per_seq << a.kv.page_shift || (a.rope && pos >= a.n_rope)) {
+    flag_error(DEV_ERR_BAD_ARG);
+    return;
   }
+  T* dst;
+  if (is_q) {
+    dst = static_cast<T*>(a.q_out) + (row * a.n_heads + head) * a.hd;
+  } else {
+    const int page = a.kv.table[seq * a.kv.table_stride + (pos >> a.kv.page_shift)];
+    if ((unsigned)page >= (unsigned)a.kv.n_pages) {
+      flag_error(DEV_ERR_BAD_ARG);
+      return;
+    }
+    dst = reinterpret_cast<T*>(const_cast<char*>(is_v ? a.kv.v : a.kv.k) + page_row(a.kv, page, pos) +
+                               (is_v ? head - nq - a.n_kv : head - nq) * a.kv.head_stride);
+  }
+  if (a.rope && !is_v) {
+    float cs[N];
+    load_vec<float, float>(a.rope + (long long)pos * a.hd + d, cs);
+#pragma unroll
+    for (int k = 0; k < N; k += 2) {
+      const float x0 = x[k], x1 = x[k + 1], c = cs[k], s = cs[k + 1];
+      x[k] = __fsub_rn(__fmul_rn(x0, c), __fmul_rn(x1, s));
+      x[k + 1] = __fadd_rn(__fmul_rn(x0, s), __fmul_rn(x1, c));
+    }
+  }
+  store_vec(dst + d, x);
 }
 
 cudaError_t launch_paged_append(int in_type, int type, const AppendArgs& a, cudaStream_t st) {
   const int n = type == F32 ? 4 : 8;
-  const long long items = a.rows * ((a.q ? a.n_heads : 0) + 2 * a.n_kv) * (a.hd / n), blocks = (items + 255) / 256;
-  const long long most = (long long)sm_count(current_device()) * 8 * 8;  // 8 waves of resident CTAs, then a loop
-  const unsigned grid = (unsigned)(blocks < most ? blocks : most);
+  const dim3 grid((unsigned)a.rows, (((a.q ? a.n_heads : 0) + 2 * a.n_kv) * (a.hd / n) + 255) / 256);  // y <= 9216: heads are checked
 #define VTB_APP(X, T) paged_append_kernel<X, T><<<grid, 256, 0, st>>>(a)
   if (type == F32) VTB_APP(float, float);
   else if (type == T_F16 && in_type == F32) VTB_APP(float, __half);
