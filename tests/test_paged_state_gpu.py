@@ -215,3 +215,22 @@ def test_bad_paged_calls(model):
         st.release(0)
     st.reset()
     assert st.free_pages() == 8
+
+
+def test_fork_shares_only_written_pages(model):
+    """A begun token that is given up leaves its page with the sequence; a fork must not share it."""
+    m, _ = model
+    st, want = CudaState(m, 2, 64, paged=PagedConfig(16, 16)), CudaState(m, 2, 64, paged=PagedConfig(16, 16))
+    for s in (st, want):
+        s.prefill(tokens(16, 1), 1)                   # whole pages: the next token opens one
+    st.lib.vtb_cuda_begin_token(st.h, np.array([4, 5], np.int32).ctypes.data)
+    st.prefill(tokens(3, 2), 0)                       # ends the begun token
+    for s in (st, want):
+        s.fork(0, 1)
+    for i in range(4):
+        t = np.array([7 + i, 90 + i], np.int32)       # the two go on differently
+        la, _ = st.step(t)
+        lb, _ = want.step(t)
+        assert np.array_equal(la, lb)
+    assert not np.array_equal(la[0], la[1])
+    ops.check_device_error()

@@ -1436,7 +1436,7 @@ int vtb_cuda_state_fork(VtbCudaState* s, int32_t dst, int32_t src) {
   cudaSetDevice(s->device);
   PagePool* p = s->pool;
   const int64_t pos = s->seq_pos[src];
-  const int last = (int)(pos / p->c.page_size);
+  const int last = (int)(pos / p->c.page_size);  // (src may hold pages behind it, for a token that was begun and given up)
   const bool tail = pos % p->c.page_size != 0;
   // The page for the copy is found before anything changes: a free one, or one that only dst holds.
   if (tail && p->free_ids.empty()) {
@@ -1445,9 +1445,9 @@ int vtb_cuda_state_fork(VtbCudaState* s, int32_t dst, int32_t src) {
     if (!gives) return merr(VTB_CUDA_ERR_STREAM_ABORTED, "KV cache pages exhausted");
   }
   pool_drop_seq(p, dst);
-  for (int i = 0; i < p->per; ++i) {
+  for (int i = 0; i < last; ++i) {
     const int32_t e = p->at(src, i);
-    if (e < 0 || (tail && i == last)) continue;
+    if (e < 0) continue;
     p->at(dst, i) = e;
     ++p->refs[e];
   }
