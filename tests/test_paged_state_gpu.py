@@ -234,3 +234,21 @@ def test_fork_shares_only_written_pages(model):
         assert np.array_equal(la, lb)
     assert not np.array_equal(la[0], la[1])
     ops.check_device_error()
+
+
+def test_bad_token_in_a_later_chunk(model):
+    """The chunks before it count, and the state goes on from there."""
+    m, _ = model
+    st, want = CudaState(m, 2, 16, paged=PagedConfig(16, 16)), CudaState(m, 2, 16, paged=PagedConfig(16, 16))
+    t = tokens(40, 3)
+    want.prefill(t[:16], 0)
+    t[20] = SMALL.vocab_size
+    with pytest.raises(_lib.VtbError):
+        st.prefill(t, 0)
+    assert st.pos(0) == 16
+    st.fork(1, 0)                                     # nothing is being computed
+    want.fork(1, 0)
+    la, lb = st.step(np.array([5, 6], np.int32))[0], want.step(np.array([5, 6], np.int32))[0]
+    assert np.array_equal(la, lb)
+    st.release(0)
+    assert st.pos(0) == 0

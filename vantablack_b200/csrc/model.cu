@@ -1993,7 +1993,10 @@ int vtb_cuda_prefill(VtbCudaState* s, int32_t seq, const int32_t* tokens, int32_
     std::vector<int32_t> sq(rows, seq), pos(rows);
     for (int r = 0; r < rows; ++r) pos[r] = (int32_t)(s->seq_pos[seq] + r);
     int rc = stage_rows(s, rows, tokens + done, sq.data(), pos.data());
-    if (rc) return rc;
+    if (rc) {
+      if (done) s->rows = 0;  // the chunks before are done: nothing is being computed
+      return rc;
+    }
     cudaError_t e = upload_table(s);
     if (e == cudaSuccess) e = enqueue_embed(s);
     for (int l = 0; l < c.n_layers && e == cudaSuccess; ++l) e = enqueue_layer(s, l);
