@@ -146,3 +146,20 @@ def test_packed_descriptors_have_the_c_layout(lib):
         vals = [0.5 if t is C.c_float else i + 1 for i, (_, t) in enumerate(c._fields_)]
         got = c.from_buffer_copy(packed.pack(*vals))
         assert [getattr(got, n) for n, _ in c._fields_] == vals
+
+
+def test_counts_that_would_overflow_are_refused(lib, buf):
+    p = buf[1]
+    kv, a = kv_args(p), attn_args(p, lib)
+    assert lib.vtb_cuda_paged_attn_prefill(C.byref(kv), C.byref(a), p, 1 << 62, None) == -1  # 4 heads a group: 2^64
+    many = (1 << 31) - 1
+    assert lib.vtb_cuda_paged_copy(C.byref(kv), many, 0, p, p, many, None, None, None) != 0
+    kv = kv_args(p, n_kv_heads=4096, page_size=1024)
+    assert lib.vtb_cuda_paged_copy(C.byref(kv), many, 0, p, p, many, None, None, None) != 0
+
+
+def test_empty_list_of_rows_needs_no_address(lib, buf):
+    p = buf[1]
+    kv, a = kv_args(p), attn_args(p, lib, q=None, out=None)
+    assert lib.vtb_cuda_paged_attn_prefill(C.byref(kv), C.byref(a), p, 0, None) == 0
+    assert lib.vtb_cuda_paged_attn_prefill(C.byref(kv), C.byref(a), p, 1, None) == -1

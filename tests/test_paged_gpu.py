@@ -513,3 +513,104 @@ def test_prompt_fork_decode_compact(dtype):
     for _ in range(3):
         step([1, 1])
     step([7, 2])
+
+
+def test_no_sequences_and_no_rows():
+    cache = P.Cache([20, 3], 2, 64, 16, BF16, 61)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    none = torch.empty(0, 8, 64, dtype=BF16, device="cuda")
+    got = ops.paged_attention_decode(none, cache.k, cache.v, cache.table[:0], cache.d_lens[:0])
+    assert got.shape == none.shape
+    got = ops.paged_attention_prefill(none, cache.k, cache.v, cache.table, cache.d_lens, i32([0, 0, 0]))
+    assert got.shape == none.shape
+    got = ops.paged_attention_prefill(none, cache.k, cache.v, cache.table[:0], cache.d_lens[:0], i32([0]))
+    assert got.shape == none.shape
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_longest_window_and_sinks(dtype):
+    """The largest window and sinks an int holds see what no window sees; rows before the first position give zeros."""
+    cache = P.Cache([150, 9], 2, 64, 16, dtype, 62)
+    top = 2 ** 31 - 1
+    for w, n in ((top, 0), (top, top), (1, top)):
+        q, got = run_decode(cache, 8, 64)
+        assert torch.equal(got, run_decode(cache, 8, 64, w, n)[1])
+        q, got = run_prefill(cache, [140, 9], 8, 64)
+        if w == top:
+            assert torch.equal(got, run_prefill(cache, [140, 9], 8, 64, w, n)[1])
+        else:
+            run_prefill(cache, [140, 9], 8, 64, w, n)
+    q = torch.randn(40, 8, 64, device="cuda").to(dtype)
+    starts = torch.tensor([0, 0, 40], dtype=torch.int32, device="cuda")
+    want = ops.paged_attention_prefill(q, cache.k, cache.v, cache.table, cache.d_lens, starts)
+    got = ops.paged_attention_prefill(q, cache.k, cache.v, cache.table, cache.d_lens, starts, window=top, sinks=top)
+    assert torch.equal(got, want) and not got[:31].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_captured_chunk_step(dtype):
+    """Append and chunk attention in one captured graph, first called there, replayed with other rows, positions and
+    lengths; a second graph with its own workspace runs in between."""
+    heads, kv, hd, page, n = 12, 4, 64, 8, 37
+    cache = P.Cache([400, 300], kv, hd, page, dtype, 63)
+    g = torch.Generator().manual_seed(64)
+    side, graphs = torch.cuda.Stream(), []
+    for _ in range(2):
+        rows = torch.zeros(n, heads + 2 * kv, hd, device="cuda")
+        seq, pos = (torch.zeros(n, dtype=torch.int32, device="cuda") for _ in range(2))
+        lens, starts = torch.zeros(2, dtype=torch.int32, device="cuda"), torch.zeros(3, dtype=torch.int32, device="cuda")
+        out = torch.empty(n, heads, hd, dtype=dtype, device="cuda")
+        ws = ops.paged_attention_workspace(dtype, heads, kv, hd)
+        q = torch.empty(n, heads, hd, dtype=dtype, device="cuda")
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            ops.paged_append(cache.k, cache.v, cache.table, rows[:, heads:heads + kv], rows[:, heads + kv:], seq, pos,
+                             q=rows[:, :heads], q_out=q)
+            ops.paged_attention_prefill(q, cache.k, cache.v, cache.table, lens, starts, out=out, workspace=ws)
+        graphs.append((graph, rows, seq, pos, lens, starts, out, q))
+    for turn, (first, counts) in enumerate([((300, 40), (20, 17)), ((0, 263), (0, 37)), ((50, 7), (36, 1)), ((363, 0), (37, 0))]):
+        graph, rows, seq, pos, lens, starts, out, q = graphs[turn % 2]
+        x = torch.randn(n, heads + 2 * kv, hd, generator=g)
+        rows.copy_(x)
+        seq.copy_(torch.tensor([s for s in range(2) for _ in range(counts[s])], dtype=torch.int32))
+        pos.copy_(torch.tensor([first[s] + i for s in range(2) for i in range(counts[s])], dtype=torch.int32))
+        now = [first[s] + counts[s] for s in range(2)]
+        lens.copy_(torch.tensor(now, dtype=torch.int32))
+        starts.copy_(torch.tensor([0, counts[0], n], dtype=torch.int32))
+        graph.replay()
+        torch.cuda.synchronize()
+        at = 0
+        for s in range(2):
+            c = counts[s]
+            cache.k_rows[s][first[s]:now[s]] = x[at:at + c, heads:heads + kv].to(dtype)
+            cache.v_rows[s][first[s]:now[s]] = x[at:at + c, heads + kv:].to(dtype)
+            if c:
+                ref, a, b = P.attention(q[at:at + c].double().cpu(), cache.k_rows[s][:now[s]].double(),
+                                        cache.v_rows[s][:now[s]].double(), torch.arange(first[s], now[s]), hd ** -0.5)
+                tol = P.attention_tolerance(ref, a, b, now[s], dtype, P_ROUNDED["prefill"])
+                assert bool(((out[at:at + c].double().cpu() - ref).abs() <= tol).all())
+            at += c
+    ops.check_device_error()
+
+
+def test_default_workspaces_on_two_streams():
+    """Calls without a workspace of their own on two streams at once, chunk and single-token attention."""
+    caches = [P.Cache([1900, 40], 2, 128, 64, BF16, 70 + i) for i in range(2)]
+    qd = [torch.randn(2, 8, 128, device="cuda").to(BF16) for _ in range(2)]
+    qp = [torch.randn(50, 8, 128, device="cuda").to(BF16) for _ in range(2)]
+    starts = torch.tensor([0, 30, 50], dtype=torch.int32, device="cuda")
+    call = lambda i: (ops.paged_attention_decode(qd[i], caches[i].k, caches[i].v, caches[i].table, caches[i].d_lens),  # noqa: E731
+                      ops.paged_attention_prefill(qp[i], caches[i].k, caches[i].v, caches[i].table, caches[i].d_lens, starts))
+    want = [call(i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = [[], []]
+    for _ in range(20):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(call(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(d, want[i][0]) and torch.equal(p, want[i][1]) for d, p in outs[i])
+    ops.check_device_error()

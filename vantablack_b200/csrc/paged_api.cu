@@ -1,6 +1,6 @@
 // paged_api.cu -- extern "C" entry points of the paged key-value cache:
-// argument checks, then one launch (two for a decode call whose sequences are
-// cut).  Included after api.cu, paged_cache.cu and paged_attn.cu.
+// argument checks, then one launch (two for an attention call whose sequences are
+// split over CTAs).  Included after api.cu and the paged kernels.
 
 static int paged_elem_bytes(int type) { return type == F32 ? 4 : type == T_F16 || type == T_BF16 ? 2 : 0; }
 static bool mul16(long long elems, int es) { return elems * es % 16 == 0; }
@@ -32,6 +32,7 @@ static int paged_view(const VtbCudaPagedKv* kv, bool need_table, PagedView* out)
 }
 
 static int paged_rows_ok(const void* p, int64_t n, int64_t row, int64_t head, int es, int64_t hd) {
+  if (n == 0) return VTB_CUDA_OK;  // (an empty list may have no address)
   if (!p) return set_err(VTB_CUDA_ERR_INVALID_ARG, "null rows");
   if (!aligned16(p) || !mul16(row, es) || !mul16(head, es) || row < (n > 1 ? hd : 0) || head < hd || row > (int64_t(1) << 40) ||
       head > (int64_t(1) << 40))
@@ -70,8 +71,9 @@ static int paged_attn_args(const VtbCudaPagedKv* kv, const VtbCudaPagedAttn* p, 
   a->rows = kv->n_seqs;
   a->n_kv = kv->n_kv_heads;
   a->group = p->n_heads / kv->n_kv_heads;
-  a->window = p->window;
-  a->sinks = p->sinks;
+  // positions lie below 2^30: a longer window sees the same, and nothing overflows
+  a->window = p->window < (1 << 30) ? p->window : 1 << 30;
+  a->sinks = p->sinks < (1 << 30) ? p->sinks : 1 << 30;
   a->tile = a->recip = 0;
   a->negate = false;
   a->scale2 = (float)((double)p->scale * 1.4426950408889634);
@@ -102,7 +104,7 @@ int vtb_cuda_paged_attn_prefill(const VtbCudaPagedKv* kv, const VtbCudaPagedAttn
   AttnArgs a;
   int rc = paged_attn_args(kv, p, n_rows, &a);
   if (rc) return rc;
-  if (!starts || n_rows < 0 || n_rows * a.group > INT_MAX || kv->n_kv_heads > 65535)
+  if (!starts || n_rows < 0 || n_rows > INT_MAX / a.group)
     return set_err(VTB_CUDA_ERR_INVALID_ARG, "bad starts or n_rows");
   if (n_rows == 0) return VTB_CUDA_OK;
   a.starts = starts;

@@ -180,6 +180,7 @@ __global__ void __launch_bounds__(CP_THREADS) paged_copy_kernel(const __grid_con
 
 cudaError_t launch_paged_copy(CopyArgs a, cudaStream_t st) {
   a.chunks = (a.page_pieces + CP_THREADS * CP_DEPTH - 1) / (CP_THREADS * CP_DEPTH);
+  if ((double)a.moves * a.n_layers * 2 * a.chunks > 2147483647.) return cudaErrorInvalidValue;  // (before it overflows)
   a.copy_blocks = a.moves * a.n_layers * 2 * a.chunks;
   long long extra = a.table ? (a.table_rows * a.table_cols + CP_THREADS - 1) / CP_THREADS : 0;
   if (extra > sm_count(current_device())) extra = sm_count(current_device());

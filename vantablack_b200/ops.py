@@ -305,6 +305,8 @@ def paged_attention_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     kv, dev, dt, shape, n_seqs = _paged_kv(k_pages, v_pages, page_table)
     if q.shape[0] != n_seqs:
         raise ValueError("q must have one row per sequence")
+    if n_seqs == 0:
+        return torch.empty_like(q) if out is None else out
     out, a, workspace = _attn(q, k_pages, dev, dt, shape, n_seqs, lens, scale, window, sinks, out, workspace)
     _lib.check(lib.vtb_cuda_paged_attn_decode(kv, a, _stream_of(dev)), "vtb_cuda_paged_attn_decode")
     return out
@@ -319,6 +321,8 @@ def paged_attention_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: tor
     in the pages already (paged_append).  Rows that no sequence holds are left as they were."""
     kv, dev, dt, shape, n_seqs = _paged_kv(k_pages, v_pages, page_table)
     at = _vec(starts, "starts", dev, n_seqs + 1)
+    if q.shape[0] == 0:
+        return torch.empty_like(q) if out is None else out
     out, a, workspace = _attn(q, k_pages, dev, dt, shape, n_seqs, lens, scale, window, sinks, out, workspace)
     _lib.check(lib.vtb_cuda_paged_attn_prefill(kv, a, at, q.shape[0], _stream_of(dev)), "vtb_cuda_paged_attn_prefill")
     return out
