@@ -21,8 +21,10 @@
 // dimension, so that it writes 16-byte pieces of positions).  The next tile's K
 // and V wait in registers until the products of this one have read the shared
 // tiles.
-// Tensor work: 72 instructions, 3072 clocks per tile at the tf32 rate; the
-// softmax and its hand-overs come on top, as TMEM has no room for a second S.
+// Tensor work of a tile at 128 values: 48 instructions of Q K^T (46 clocks each,
+// measured) and 24 of P V (67), 3.8k clocks; a tile takes 8.5k, as the softmax with
+// its splits follows Q K^T and TMEM has no room for a second S.  256 tokens on 1797
+// (32 / 8 heads x 128): 97 to 100 us, 83 TFLOP/s, 250 in tf32 products.
 #include <type_traits>
 
 #include "paged.cuh"
