@@ -614,3 +614,37 @@ def test_default_workspaces_on_two_streams():
     for i in range(2):
         assert all(torch.equal(d, want[i][0]) and torch.equal(p, want[i][1]) for d, p in outs[i])
     ops.check_device_error()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("page", [2, 16])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (70, 5)])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_prefill_infinities_and_nans_of_v_reach_their_values_only(dtype, page, window, sinks, value):
+    """One value of some V rows is not finite: the queries that see it get it in that value, every other value is as if
+    it were 0.  (Sequence 0: 210 new tokens on 40, also split over CTAs by a call of its own; the bad rows lie before the
+    chunk, inside it and at its end.)"""
+    cache = P.Cache([250, 1300], 2, 64, page, dtype, 36)
+    at = [2, 45, 100, 101, 233, 249]
+    for t in at:
+        cache.v[int(cache.table[0, t // page]), 1, t % page, 5] = value
+        cache.v_rows[0][t, 1, 5] = 0.0
+    g = torch.Generator().manual_seed(3)
+    q = torch.randn(211, 8, 64, generator=g).to(dtype).cuda()
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    got = ops.paged_attention_prefill(q, cache.k, cache.v, cache.table, cache.d_lens, i32(0, 210, 211), window=window, sinks=sinks)
+    alone = ops.paged_attention_prefill(q[205:210], cache.k, cache.v, cache.table[:1], cache.d_lens[:1], i32(0, 5),
+                                        window=window, sinks=sinks)
+    ops.check_device_error()
+    for out, first in ((got[:210], 40), (alone, 245)):
+        pos = torch.arange(first, 250)
+        see = P.visible(pos, torch.tensor(at), window, sinks).any(1)
+        x = out.double().cpu()
+        ref, a, b = P.attention(q[first - 40:210].double().cpu(), cache.k_rows[0].double(), cache.v_rows[0].double(), pos, 0.125,
+                                window, sinks)
+        ok = (x - ref).abs() <= P.attention_tolerance(ref, a, b, 250, dtype, P_ROUNDED["prefill"])
+        bad = x[see][:, 4:, 5]  # kv head 1's queries that see one
+        assert bool(torch.isnan(bad).all()) if math.isnan(value) else bool((bad == value).all())
+        ok[:, 4:, 5] |= see[:, None]
+        assert bool(ok.all())
+    check_rows(got[210:], cache, 1, q[210:], torch.tensor([1299]), 0.125, window, sinks, "prefill")

@@ -51,7 +51,7 @@ template <int HD> struct F32Prefill {
 struct F32Bars {
   uint64_t q_full, k_full, k_freed, v_full, v_freed, s_full, p_full, o_full;
   uint32_t tmem;
-  int by_rows;  // a V row that may be hidden from some query rows is infinite or NaN (attend_row)
+  int bad0, bad1;  // tiles with infinities or NaN in V lie in [bad0, bad1) (add_nonfinite)
 };
 
 template <int HD>
@@ -76,7 +76,8 @@ __global__ void __launch_bounds__(F_THREADS, 1) paged_prefill_f32_kernel(const _
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&bar.tmem)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   } else if (threadIdx.x == 0) {
-    bar.by_rows = 0;
+    bar.bad0 = 0x7fffffff;
+    bar.bad1 = 0;
     mbar_init(&bar.q_full, 4);
     mbar_init(&bar.k_full, 4);
     mbar_init(&bar.v_full, 4);
@@ -207,11 +208,22 @@ __global__ void __launch_bounds__(F_THREADS, 1) paged_prefill_f32_kernel(const _
           x[i] = *reinterpret_cast<const float*>(a.kv.v + off + d * 4);
         }
       };
-      bool odd = false;
       if (n > 0) fetch(0);
       for (int j = 0; j < n; ++j) {
         if (j) ok = warp_wait(&bar.v_freed, (j - 1) & 1);
         if (!ok) break;
+        bool odd = false;
+#pragma unroll
+        for (int i = 0; i < POS; ++i) odd |= (__float_as_uint(x[i]) & 0x7f800000u) == 0x7f800000u;
+        if (__any_sync(0xffffffffu, odd)) {
+#pragma unroll
+          for (int i = 0; i < POS; ++i)
+            if ((__float_as_uint(x[i]) & 0x7f800000u) == 0x7f800000u) x[i] = 0.f;
+          if (lane == 0) {
+            atomicMin(&bar.bad0, j);
+            atomicMax(&bar.bad1, j + 1);
+          }
+        }
 #pragma unroll
         for (int i = 0; i < POS; i += 4) {
           const int pc = (p0 + i) / 4;  // 16-byte piece of the row of dimension d
@@ -220,13 +232,11 @@ __global__ void __launch_bounds__(F_THREADS, 1) paged_prefill_f32_kernel(const _
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const float v = (j0 + j) * FN + p0 + i + c < sp.n ? x[i + c] : 0.f;
-            odd |= (__float_as_uint(v) & 0x7f800000u) == 0x7f800000u;
             split_tf32(v, hi[c], lo[c]);
           }
           st4(at, hi);
           st4(at + C::KV, lo);
         }
-        if (__any_sync(0xffffffffu, odd) && lane == 0) bar.by_rows = 1;
         landed(&bar.v_full);
         if (j + 1 < n) fetch(j + 1);
       }
@@ -354,17 +364,15 @@ __global__ void __launch_bounds__(F_THREADS, 1) paged_prefill_f32_kernel(const _
     // ---------------- output: whole rows through shared memory ----------------
     if (ok) {
       float* part = a.part + (long long)blockIdx.x * C::SLOT;
-      if (n > 0 && *reinterpret_cast<volatile int*>(&bar.by_rows) && row) {
-        float acc[HD];
-        for (int i = 0; i < HD; ++i) acc[i] = 0.f;
-        m = -INFINITY;
-        l = 0.f;
-        const int t = a.token(r), head = kvh * a.group + r - t * a.group;
-        const float* q = static_cast<const float*>(a.q) + (rt.r0 + tok0 + t) * a.q_row + head * a.q_head;
-        for (int i = j0 * FN; i < min((j0 + n) * FN, sp.n); ++i)
-          attend_row<float, HD>(a, rt.s, kvh, q, rt.ctx + tok0 + t, sp.pos(i), sp.pos(i) + 1, m, l, acc);
+      const int bad0 = *reinterpret_cast<volatile int*>(&bar.bad0), bad1 = *reinterpret_cast<volatile int*>(&bar.bad1);
+      if (bad0 < bad1 && row) {
+        float x[HD];
 #pragma unroll
-        for (int i = 0; i < HD; ++i) o[i] = acc[i];
+        for (int i = 0; i < HD; ++i) x[i] = o[i];
+        for (int i = (j0 + bad0) * FN; i < min((j0 + bad1) * FN, vc); ++i)
+          if (i < va || i >= vb) add_nonfinite<float, HD>(a, rt.s, kvh, sp.pos(i), 0, x);
+#pragma unroll
+        for (int i = 0; i < HD; ++i) o[i] = x[i];
       }
       const float inv = splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
       __syncwarp();

@@ -20,8 +20,8 @@
 // by TMA, K and V into two stages each, one box per page and 64 values (4-d map
 // over the page pool); 9 and 11: in tiles at an edge (the last positions, the
 // window's start) put zeros in place of V rows at positions that no query row
-// sees, so that what lies in the rest of a page never meets P = 0, and look for
-// infinities and NaN in the others (attend_row).  Pages of fewer than 8 positions,
+// sees, so that what lies in the rest of a page never meets P = 0, and in place of
+// infinities and NaN in the others (add_nonfinite).  Pages of fewer than 8 positions,
 // whose boxes would break the swizzle, are gathered row by row with cp.async by
 // warps 9 to 11.
 //
@@ -30,7 +30,7 @@
 // hand-overs, 3440 per tile of 128 positions where the tensor cores need 2048 for
 // both row tiles.  Measured (32 / 8 heads x 128, bf16): 2048 tokens 51 us (0.67
 // PFLOP/s), 8192 under a window of 4096 437 to 456 us (0.93); 11 chunks of 1 to 511
-// (32 / 4 x 64, f16) 88 us.  P in columns of its own at 64 values, so that the next
+// (32 / 4 x 64, f16) 90 us.  P in columns of its own at 64 values, so that the next
 // Q K^T need not wait for P V, gave nothing (3370 clocks to 3570 to 3740).
 //
 // The scale is taken positive (a negative one negates Q in the first product),
@@ -113,25 +113,24 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// Rows one by one, for tiles in which a V row that only part of the query rows
-// see holds an infinity or a NaN: 0 * inf in the tile products would carry it to
-// the rows that do not see it.  Adds the positions [t0, t1) that a query at
-// position p sees to (m, l, acc), in f32.
-template <typename T, int HD>
-__device__ __noinline__ void attend_row(const AttnArgs& a, int s, int kvh, const T* q, int p, int t0, int t1, float& m, float& l,
-                                        float* acc) {
-  const int32_t* table = a.kv.table + s * a.kv.table_stride;
-  for (int t = t0; t < t1 && t <= p; ++t) {
-    if (a.window && t <= p - a.window && t >= a.sinks) continue;
-    const long long off = page_row(a.kv, __ldg(table + (t >> a.kv.page_shift)), t) + kvh * a.kv.head_stride;
-    const T *k = reinterpret_cast<const T*>(a.kv.k + off), *v = reinterpret_cast<const T*>(a.kv.v + off);
-    float x = 0.f;
-    for (int d = 0; d < HD; ++d) x = fmaf(to_f(q[d]), to_f(k[d]), x);
-    x *= a.negate ? -a.scale2 : a.scale2;
-    const float mn = fmaxf(m, x), b = mn == -INFINITY ? 0.f : mn, f = exp2f(m - b), e = exp2f(x - b);
-    m = mn;
-    l = l * f + e;
-    for (int d = 0; d < HD; ++d) acc[d] = acc[d] * f + e * to_f(v[d]);
+// A V row that only part of a tile's query rows see may hold infinities or NaN:
+// 0 * inf in the tile products would carry them to the rows that do not see it.
+// So zeros go into the products in their place, and the rows that do see the
+// position get them here, value by value (inf + x = inf, whatever P is).  An infinity
+// in the last of 2048 tokens on 32768: 1.07 -> 1.47 ms; what the look for them costs
+// where there are none is 0 to 3%.
+// Adds the infinite and NaN ones of values [d0, d0 + N) of V at position t to o.
+template <typename T, int N>
+__device__ __noinline__ void add_nonfinite(const AttnArgs& a, int s, int kvh, int t, int d0, float* o) {
+  const int page = __ldg(a.kv.table + s * a.kv.table_stride + (t >> a.kv.page_shift));
+  const T* v = reinterpret_cast<const T*>(a.kv.v + page_row(a.kv, page, t) + kvh * a.kv.head_stride) + d0;
+  constexpr int PER = 16 / sizeof(T);
+  for (int d = 0; d < N; d += PER) {
+    float x[PER];
+    load_vec<T, T>(v + d, x);
+#pragma unroll
+    for (int k = 0; k < PER; ++k)
+      if ((__float_as_uint(x[k]) & 0x7f800000u) == 0x7f800000u) o[d + k] += x[k];
   }
 }
 // Whether one of the 16-bit values in w is infinite or NaN, in bits 15 and 31 of the result.
@@ -158,14 +157,18 @@ struct TcBars {
   uint64_t next_full[2], next_read[2];
   uint64_t q_full, q_freed, k_full[2], k_freed[2], v_full[2], v_freed[2], v_raw[2], s_full[2], p_full[2], o_full[2], done;
   uint32_t tmem;
-  int rows_of[4];  // [i & 3] = i + 1: the CTA's i-th item is to be done row by row
+  int mended[4];  // [i & 3] = i + 1: the CTA's i-th item has zeros in place of infinities or NaN in V
 };
 
 // One piece of work: two row tiles of a kv head over one split of the positions they see.
 struct TcItem {
   RowTile rt;
-  int kvh, nflat, p1, w0, ks, kw, j0, na, nb;
+  int kvh, nflat, first, p1, w0, ks, kw, j0, na, nb;  // first: position of the first row (p1: of the last)
   __device__ __forceinline__ int tiles() const { return max(na, nb); }
+  // Whether some of the item's rows do not see all of the tile at t0.
+  __device__ __forceinline__ bool edge(int t0, const AttnArgs& a) const {
+    return t0 + TN > first + 1 || (a.window && t0 < p1 + 1 - a.window);
+  }
   __device__ __forceinline__ int pos(int j) const { return (j0 + j < ks ? j0 + j : j0 + j - ks + kw) * TN; }  // first of tile j
 };
 // Item `i` of `items`: (row tile from the last, kv head, split), so the longest rows
@@ -178,7 +181,8 @@ __device__ __forceinline__ bool tc_item(const AttnArgs& a, int i, int items, int
   t.nflat = rt.n * a.group;
   // Positions [w0, p1] and, when a window has left them behind, the first `sinks`
   // of [0, w0), in tiles at multiples of TN: `ks` sink tiles, then those from kw.
-  const int last = min(rt.f0 + 2 * a.tile, t.nflat) - 1, p0 = max(0, rt.ctx + rt.f0 / a.group);
+  t.first = rt.ctx + rt.f0 / a.group;
+  const int last = min(rt.f0 + 2 * a.tile, t.nflat) - 1, p0 = max(0, t.first);
   t.p1 = rt.ctx + last / a.group;
   t.w0 = a.window && p0 >= a.window ? p0 + 1 - a.window : 0;
   t.kw = t.w0 / TN;
@@ -231,7 +235,7 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&bar.tmem)));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   } else if (threadIdx.x == 0) {
-    for (int i = 0; i < 4; ++i) bar.rows_of[i] = 0;
+    for (int i = 0; i < 4; ++i) bar.mended[i] = 0;
     mbar_init(&bar.q_full, 1);
     mbar_init(&bar.q_freed, 1);
     mbar_init(&bar.done, 1);
@@ -373,9 +377,8 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
         if (!any) continue;
         const RowTile& rt = it.rt;
         const int32_t* table = a.kv.table + rt.s * a.kv.table_stride;
-        const int n = it.tiles(), p1 = it.p1, w0 = it.w0, first = rt.ctx + rt.f0 / a.group;
+        const int n = it.tiles(), p1 = it.p1, w0 = it.w0;
         ++ni;
-        uint32_t odd = 0;  // nonfinite2 of V rows that only part of the item's rows see
         if (warp == 10) {  // Q: both tiles, a box of (64 values, group, tokens of a tile) each
           if (nq) ok = warp_wait(&bar.q_freed, (nq - 1) & 1);
           if (!ok) break;
@@ -420,13 +423,25 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
           }
           cpa_commit();
         };
-        auto look = [&](uint32_t at) {
-          uint32_t x[4];
-          asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
-          odd |= nonfinite2<T>(x[0]) | nonfinite2<T>(x[1]) | nonfinite2<T>(x[2]) | nonfinite2<T>(x[3]);
-        };
-        auto report = [&]() {
-          if (__any_sync(0xffffffffu, odd & 0x80008000u) && lane == 0) bar.rows_of[ni & 3] = ni + 1;
+        // V rows of an edge tile in shared memory, this lane's piece of row r at place(r): zeros in place of infinities and NaN
+        auto look = [&](auto place, int r0, auto rounds, int step) {
+          uint32_t odd = 0, x[4];
+          auto get = [&](uint32_t at) {
+            asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at) : "memory");
+            return nonfinite2<T>(x[0]) | nonfinite2<T>(x[1]) | nonfinite2<T>(x[2]) | nonfinite2<T>(x[3]);
+          };
+#pragma unroll 8
+          for (int i = 0; i < rounds; ++i) odd |= get(place(r0 + i * step));
+          if (!__any_sync(0xffffffffu, odd & 0x80008000u)) return;
+          if (lane == 0) bar.mended[ni & 3] = ni + 1;
+#pragma unroll 1
+          for (int i = 0; i < rounds; ++i)
+            if (get(place(r0 + i * step)) & 0x80008000u) {
+#pragma unroll
+              for (int c = 0; c < 4; ++c) x[c] &= ~(((nonfinite2<T>(x[c]) & 0x80008000u) >> 15) * 0xffffu);
+              asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};"
+                           ::"r"(place(r0 + i * step)), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]) : "memory");
+            }
         };
         for (int j = 0; j < n; ++j, ++kt) {
           if (warp == 10 && j + 1 == n) request(k);
@@ -449,10 +464,11 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
             cpa_wait<1>();
             landed(&bar.k_full[slot]);
             cpa_wait<0>();
-            for (int r = (warp - 9) * RPW + sub; r < TN; r += 3 * RPW) look(av + (pc >> 3) * C::ATOM + r * 128 + (((pc & 7) ^ (r & 7)) << 4));
-            report();
+            if (it.edge(t0, a))
+              look([&](int r) { return av + (pc >> 3) * C::ATOM + r * 128 + (((pc & 7) ^ (r & 7)) << 4); }, (warp - 9) * RPW + sub,
+                   (TN - ((warp - 9) * RPW + sub) + 3 * RPW - 1) / (3 * RPW), 3 * RPW);
             landed(&bar.v_full[slot]);
-          } else if (t0 + TN > first + 1 || (a.window && t0 < p1 + 1 - a.window)) {
+          } else if (it.edge(t0, a)) {
             // an edge tile: zeros in place of the V rows that no query row sees, and a look at the others
             if (warp == 10) {
               if (lane == 0) mbar_arrive(&bar.v_full[slot]);
@@ -469,9 +485,8 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
                     *reinterpret_cast<uint4*>(smem + (4 + slot) * C::TILE + (pc >> 3) * C::ATOM + r * 128 + ((pc & 7) << 4)) =
                         make_uint4(0, 0, 0, 0);
                 }
-#pragma unroll 8
-              for (int i = 0; i < TN / 2; i += RPW) look(av + (pc >> 3) * C::ATOM + (r0 + i) * 128 + ((pc & 7) << 4));
-              report();
+              look([&](int r) { return av + (pc >> 3) * C::ATOM + r * 128 + ((pc & 7) << 4); }, r0,
+                   std::integral_constant<int, TN / 2 / RPW>(), RPW);
               landed(&bar.v_full[slot]);
             }
           } else if (warp == 10) {
@@ -578,18 +593,27 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
       if (!ok) break;
       tc_fence_after();
       float* part = a.part + (long long)item * C::SLOT;
-      if (m_tiles > 0 && *reinterpret_cast<volatile int*>(&bar.rows_of[ni & 3]) == ni + 1) {
+      if (m_tiles > 0 && *reinterpret_cast<volatile int*>(&bar.mended[ni & 3]) == ni + 1) {
+        float acc[HD];
+#pragma unroll 1
+        for (int c = 0; c < HD; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(o, to + c);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) acc[c + i] = __uint_as_float(o[i]);
+        }
         if (row) {
-          float acc[HD];
-          for (int d = 0; d < HD; ++d) acc[d] = 0.f;
-          m = -INFINITY;
-          l = 0.f;
-          const int head = it.kvh * a.group + r - a.token(r) * a.group;
-          const long long tok = rt.r0 + tok0 + a.token(r);
-          for (int j = 0; j < m_tiles; ++j)
-            attend_row<T, HD>(a, rt.s, it.kvh, static_cast<const T*>(a.q) + tok * a.q_row + head * a.q_head, vc - 1, it.pos(j), it.pos(j) + TN,
-                              m, l, acc);
-          T* out = static_cast<T*>(a.out) + tok * a.o_row + head * a.o_head;
+#pragma unroll 1
+          for (int j = 0; j < m_tiles; ++j) {
+            const int t0 = it.pos(j);
+            if (!it.edge(t0, a)) continue;
+#pragma unroll 1
+            for (int t = t0; t < min(t0 + TN, vc); ++t)
+              if (t < va || t >= vb) add_nonfinite<T, HD>(a, rt.s, it.kvh, t, 0, acc);
+          }
+          const int t = a.token(r);
+          T* out = static_cast<T*>(a.out) + (rt.r0 + tok0 + t) * a.o_row + (long long)(it.kvh * a.group + r - t * a.group) * a.o_head;
           for (int d = 0; d < HD; ++d) {
             if (splits == 1) out[d] = from_f<T>(l == 0.f ? 0.f : acc[d] / l);
             else part[4 * TQ + (long long)(w * TQ + r) * HD + d] = acc[d];
