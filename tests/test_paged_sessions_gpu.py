@@ -1,0 +1,90 @@
+"""Sessions on a paged state: a windowed prompt behind queued work, prompts in chunks under a window, head_dim 128."""
+import numpy as np
+import pytest
+
+import oracle as O
+from vantablack_b200 import ops, synth as S
+from vantablack_b200.model import Context, CudaModel, CudaState, HostWeights, LlamaConfig, PagedConfig
+
+pytestmark = pytest.mark.gpu
+
+SMALL = LlamaConfig(dim=256, n_layers=2, n_heads=4, n_kv_heads=2, head_dim=64, ffn_dim=512, vocab_size=512, max_seq=128,
+                    rope_base=10000.0)
+WIDE = LlamaConfig(dim=512, n_layers=2, n_heads=4, n_kv_heads=2, head_dim=128, ffn_dim=512, vocab_size=512, max_seq=128,
+                   rope_base=10000.0)
+TALL = LlamaConfig(dim=256, n_layers=2, n_heads=4, n_kv_heads=2, head_dim=64, ffn_dim=512, vocab_size=32768, max_seq=128,
+                   rope_base=10000.0)
+LOGITS = 1e-3  # the bar of the forward loop against the oracle
+
+
+def make(cfg):
+    m = CudaModel(Context(0), HostWeights(cfg, seed=5))
+    yield m
+    m.close()
+
+
+@pytest.fixture(scope="module")
+def model():
+    yield from make(SMALL)
+
+
+def near(a, b, tol):
+    return np.abs(a - b).max() <= tol * np.abs(b).max()
+
+
+def tokens(n, seed=0):
+    return np.random.default_rng(seed).integers(3, SMALL.vocab_size, n)
+
+
+def begin(st, toks):
+    return st.lib.vtb_cuda_begin_token(st.h, np.array(toks, np.int32).ctypes.data)
+
+
+@pytest.fixture(scope="module")
+def tall():
+    yield from make(TALL)
+
+
+def test_windowed_prompt_behind_queued_work(tall):
+    """The page table goes to the device while milliseconds of work are queued before it; pages that the window leaves
+    at the end of the call are given back only when the table has been read."""
+    n = 512
+    pc = PagedConfig(n + 32, 8, S.F32, 24, 4)
+    st, want = CudaState(tall, n, n, paged=pc), CudaState(tall, 1, 128, paged=pc)
+    t = np.random.default_rng(3).integers(3, TALL.vocab_size, 100)
+    a, x = want.prefill(t)
+    assert begin(st, [5] * n) == 0
+    for _ in range(200):  # given up: about 30 us each on the device, queued faster than that
+        assert st.lib.vtb_cuda_final_step(st.h) == 0
+    b, y = st.prefill(t)
+    ops.check_device_error()
+    assert near(b, a, LOGITS) and x == y
+
+
+@pytest.mark.parametrize("kv_type", [S.F32, S.BF16])
+@pytest.mark.parametrize("page,window,sinks", [(8, 24, 0), (8, 24, 9), (16, 50, 4), (1, 17, 1)])
+def test_windowed_prompt_in_chunks(model, kv_type, page, window, sinks):
+    """A prompt in chunks of 16 rows, with pages given back between them, equals one chunk, and the steps after it."""
+    t = tokens(110, page + window)
+    pc = PagedConfig(-(-128 // page), page, kv_type, window, sinks)
+    one, cut = CudaState(model, 1, 128, paged=pc), CudaState(model, 1, 16, paged=pc)
+    tol = LOGITS if kv_type == S.F32 else 16 * 2.0 ** -8
+    a, b = one.prefill(t[:100])[0], cut.prefill(t[:100])[0]
+    assert near(b, a, tol) and cut.free_pages() == one.free_pages()
+    for tok in t[100:]:
+        assert near(cut.step([tok])[0], one.step([tok])[0], tol)
+    ops.check_device_error()
+
+
+def test_head_dim_128_against_the_oracle():
+    w = HostWeights(WIDE, seed=6)
+    m = CudaModel(Context(0), w)
+    ref, st = O.Model(w), CudaState(m, 1, 32, paged=PagedConfig(6, 16))
+    t = tokens(45, 2)
+    a, (b, y) = ref.prefill(t[:33]), st.prefill(t[:33])
+    assert near(b, a, LOGITS) and y == O.argmax(a)
+    for tok in t[33:]:
+        a, (b, y) = ref.step(int(tok)), st.step([int(tok)])
+        assert near(b[0], a, LOGITS) and y[0] == O.argmax(a)
+    ops.check_device_error()
+    m.close()

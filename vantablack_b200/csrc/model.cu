@@ -2005,17 +2005,17 @@ int vtb_cuda_prefill(VtbCudaState* s, int32_t seq, const int32_t* tokens, int32_
     if (e != cudaSuccess) return mcuda(e);
     s->seq_pos[seq] += rows;
     done += rows;
-    if (s->pool) {
-      // the next chunk's staging and table may change only when this one has been read
-      if (!last && (e = cudaStreamSynchronize(s->st))) return mcuda(e);
-      pool_evict(s->pool, seq, s->seq_pos[seq]);
-    }
     if (last) {
       s->rows = 1;
       rc = finalize(s, 1, logits, argmax);
       s->rows = 0;
-      return rc;
+    } else if (s->pool && (e = cudaStreamSynchronize(s->st))) {  // (the next chunk's staging may change now)
+      return mcuda(e);
     }
+    // Pages are given back only now that the chunk is done: the table goes to the
+    // device from the host's pinned copy, which this changes.
+    if (s->pool && rc == VTB_CUDA_OK) pool_evict(s->pool, seq, s->seq_pos[seq]);
+    if (last) return rc;
   }
   return VTB_CUDA_OK;
 }
