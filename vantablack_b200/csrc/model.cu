@@ -2009,7 +2009,7 @@ int vtb_cuda_prefill(VtbCudaState* s, int32_t seq, const int32_t* tokens, int32_
       s->rows = 1;
       rc = finalize(s, 1, logits, argmax);
       s->rows = 0;
-    } else if (s->pool && (e = cudaStreamSynchronize(s->st))) {  // (the next chunk's staging may change now)
+    } else if ((e = cudaStreamSynchronize(s->st))) {  // the next chunk's rows take the place of this one's in pinned memory
       return mcuda(e);
     }
     // Pages are given back only now that the chunk is done: the table goes to the
