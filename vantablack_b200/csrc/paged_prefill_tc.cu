@@ -21,7 +21,7 @@
 // over the page pool); 9 and 11: in tiles at an edge (the last positions, the
 // window's start) put zeros in place of V rows at positions that no query row
 // sees, so that what lies in the rest of a page never meets P = 0, and in place of
-// infinities and NaN in the others (add_nonfinite).  Pages of fewer than 8 positions,
+// infinities and NaN in the others (take_nonfinite).  Pages of fewer than 8 positions,
 // whose boxes would break the swizzle, are gathered row by row with cp.async by
 // warps 9 to 11.
 //
@@ -113,12 +113,71 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
-// A V row that only part of a tile's query rows see may hold infinities or NaN:
-// 0 * inf in the tile products would carry them to the rows that do not see it.
-// So zeros go into the products in their place, and the rows that do see the
-// position get them here, value by value (inf + x = inf, whatever P is).  An infinity
-// in the last of 2048 tokens on 32768: 1.07 -> 1.47 ms; what the look for them costs
-// where there are none is 0 to 3%.
+// Infinities and NaN in V.  0 * inf is NaN, so they may not meet the weights of rows that
+// do not see them, nor weights that are 0 only because they were rounded.  In tiles
+// that part of the rows see, zeros go into the products in their place; in the others
+// they leave a sum that is not finite.  Either way the rows that see such a position
+// get its values afterwards (inf + x = inf, whatever P is): the warp, whose rows share
+// the sequence and the kv head, looks through V 32 positions at a time and
+// visits the ones that hold any.
+// Puts them in place of what the sums x.o hold for their values.  The item sees positions
+// from w0 on and the sinks, the lane's row [0, va) and [vb, vc).
+template <int HD> struct RowSums {
+  float o[HD];
+  uint32_t set[HD / 32];  // bits of the values that such a position has given so far
+  uint32_t done;          // bits of V's 16-byte pieces whose values are all NaN: nothing changes them any more
+};
+template <typename T, int HD>
+__device__ __noinline__ void take_nonfinite(const AttnArgs& a, int s, int kvh, int t0, int t1, int w0, int va, int vb, int vc,
+                                            RowSums<HD>& x) {
+  constexpr int PER = 16 / sizeof(T), PIECES = HD / PER;
+  constexpr uint32_t ALL = 0xffffffffu >> (32 - PIECES);
+  const int32_t* table = a.kv.table + s * a.kv.table_stride;
+  const char* v = a.kv.v + kvh * a.kv.head_stride;
+  auto bad = [](float y) { return (__float_as_uint(y) & 0x7f800000u) == 0x7f800000u; };
+  for (int b = t0; b < t1; b += 32) {
+    const uint32_t skip = __reduce_and_sync(0xffffffffu, x.done);
+    if ((skip & ALL) == ALL) return;
+    const int mine = b + (threadIdx.x & 31);
+    long long off = 0;
+    uint32_t odd = 0;  // the pieces of this lane's position that hold any
+    if (mine < t1 && (mine >= w0 || mine < a.sinks)) {
+      off = page_row(a.kv, __ldg(table + (mine >> a.kv.page_shift)), mine);
+#pragma unroll 8
+      for (int p = 0; p < PIECES; ++p) {
+        float y[PER];
+        load_vec<T, T>(reinterpret_cast<const T*>(v + off) + p * PER, y);
+        bool any = false;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) any |= bad(y[k]);
+        odd |= any ? 1u << p : 0u;
+      }
+      odd &= ~skip;
+    }
+    for (unsigned hits = __ballot_sync(0xffffffffu, odd != 0); hits; hits &= hits - 1) {
+      const int l = __ffs(hits) - 1, t = b + l;
+      const long long from = __shfl_sync(0xffffffffu, off, l);
+      uint32_t m = __shfl_sync(0xffffffffu, odd, l);
+      if (t >= vc || (t < vb && t >= va)) continue;
+      for (; m; m &= m - 1) {
+        const int p = __ffs(m) - 1, d = p * PER;
+        float y[PER];
+        load_vec<T, T>(reinterpret_cast<const T*>(v + from) + d, y);
+        bool nan = true;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          if (bad(y[k])) {
+            const uint32_t bit = 1u << ((d + k) & 31);
+            x.o[d + k] = x.set[(d + k) >> 5] & bit ? x.o[d + k] + y[k] : y[k];
+            x.set[(d + k) >> 5] |= bit;
+          }
+          nan = nan && isnan(x.o[d + k]);
+        }
+        if (nan) x.done |= 1u << p;
+      }
+    }
+  }
+}
 // Adds the infinite and NaN ones of values [d0, d0 + N) of V at position t to o.
 template <typename T, int N>
 __device__ __noinline__ void add_nonfinite(const AttnArgs& a, int s, int kvh, int t, int d0, float* o) {
@@ -593,40 +652,6 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
       if (!ok) break;
       tc_fence_after();
       float* part = a.part + (long long)item * C::SLOT;
-      if (m_tiles > 0 && *reinterpret_cast<volatile int*>(&bar.mended[ni & 3]) == ni + 1) {
-        float acc[HD];
-#pragma unroll 1
-        for (int c = 0; c < HD; c += 32) {
-          uint32_t o[32];
-          tmem_ld32(o, to + c);
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) acc[c + i] = __uint_as_float(o[i]);
-        }
-        if (row) {
-#pragma unroll 1
-          for (int j = 0; j < m_tiles; ++j) {
-            const int t0 = it.pos(j);
-            if (!it.edge(t0, a)) continue;
-#pragma unroll 1
-            for (int t = t0; t < min(t0 + TN, vc); ++t)
-              if (t < va || t >= vb) add_nonfinite<T, HD>(a, rt.s, it.kvh, t, 0, acc);
-          }
-          const int t = a.token(r);
-          T* out = static_cast<T*>(a.out) + (rt.r0 + tok0 + t) * a.o_row + (long long)(it.kvh * a.group + r - t * a.group) * a.o_head;
-          for (int d = 0; d < HD; ++d) {
-            if (splits == 1) out[d] = from_f<T>(l == 0.f ? 0.f : acc[d] / l);
-            else part[4 * TQ + (long long)(w * TQ + r) * HD + d] = acc[d];
-          }
-          if (splits > 1) {
-            part[w * TQ + r] = m;
-            part[2 * TQ + w * TQ + r] = l;
-          }
-        }
-        __syncwarp();
-        tc_fence_before();
-        continue;
-      }
       const float inv = l == 0.f ? 0.f : 1.f / l;
       const uint32_t stage = sq + 6 * C::TILE + warp * 32 * 128;  // 64 values of this warp's 32 rows
       // Rows go out whole, 8 lanes to 128 bytes: this lane's rows are lane / 8 + 4 i.
@@ -640,6 +665,7 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
                        : nullptr;
         }
       }
+      f2 zero = pk(0.f, 0.f);  // 0 as long as the row's sums are finite, NaN otherwise
 #pragma unroll 1
       for (int c = 0; c < HD; c += 64) {
         uint32_t o[64];
@@ -647,6 +673,8 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
           tmem_ld32(o, to + c);
           tmem_ld32(o + 32, to + c + 32);
           tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 64; i += 2) zero = fma2(pk(__uint_as_float(o[i]), __uint_as_float(o[i + 1])), pk(0.f, 0.f), zero);
         } else {
 #pragma unroll
           for (int i = 0; i < 64; ++i) o[i] = 0u;
@@ -685,6 +713,37 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
         part[w * TQ + r] = m_tiles > 0 ? m : -INFINITY;
         part[2 * TQ + w * TQ + r] = l;
       }
+      // ---------------- infinities and NaN of V (take_nonfinite): such rows once more ----------------
+      const bool in_edges = m_tiles > 0 && *reinterpret_cast<volatile int*>(&bar.mended[ni & 3]) == ni + 1;
+      const bool in_others = __any_sync(0xffffffffu, row && l == l && hsum(zero) != 0.f);  // (a score of NaN: NaN it stays)
+      if (in_edges || in_others) {
+        RowSums<HD> x;
+        for (uint32_t& y : x.set) y = 0;
+        x.done = row ? 0u : ~0u;
+#pragma unroll 1
+        for (int c = 0; c < HD; c += 32) {
+          uint32_t o[32];
+          tmem_ld32(o, to + c);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) x.o[c + i] = __uint_as_float(o[i]);
+        }
+#pragma unroll 1
+        for (int j = 0; j < m_tiles; ++j) {
+          const int t0 = it.pos(j);
+          if (it.edge(t0, a) ? in_edges : in_others)
+            take_nonfinite<T, HD>(a, rt.s, it.kvh, t0, min(t0 + TN, it.p1 + 1), it.w0, va, vb, vc, x);
+        }
+        if (row) {
+          const int t = a.token(r);
+          T* out = static_cast<T*>(a.out) + (rt.r0 + tok0 + t) * a.o_row + (long long)(it.kvh * a.group + r - t * a.group) * a.o_head;
+          for (int d = 0; d < HD; ++d) {
+            if (splits == 1) out[d] = from_f<T>(x.o[d] * inv);
+            else part[4 * TQ + (long long)(w * TQ + r) * HD + d] = x.o[d];
+          }
+        }
+        __syncwarp();
+      }
       tc_fence_before();  // O has been read: the next item's first product (behind its P) may replace it
     }
   }
@@ -717,7 +776,7 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const __grid_co
 #pragma unroll 4
     for (int i = 0; i < splits; ++i) {
       const float* q = p + (long long)i * SLOT;
-      const float e = exp2f(q[r] - b);
+      const float e = fmaxf(exp2f(q[r] - b), 1.2e-38f);  // not 0, for the infinities of a split that weighs nothing
       L += q[ROWS + r] * e;
 #pragma unroll
       for (int k = 0; k < V; k += 4) {
