@@ -67,3 +67,16 @@ def test_prefill_infinities_where_all_rows_see_them(dtype, hd, value):
     ok = (got - ref[0]).abs() <= P.attention_tolerance(*ref, 1000, dtype, True)
     ok[:, 4:, 5] = True
     assert bool(ok.all())
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("heads,n,length,window,sinks", [(8, 700, 700, 0, 0), (6, 130, 1500, 0, 0), (4, 400, 2000, 300, 4), (2, 3, 6000, 0, 0)])
+def test_prefill_keeps_the_weights_exact(dtype, hd, heads, n, length, window, sinks):
+    """16-bit caches: the output carries its own rounding only, not one of each weight."""
+    cache = P.Cache([length], 2, hd, 16, dtype, 76)
+    q = torch.randn(n, heads, hd, generator=torch.Generator().manual_seed(9)).to(dtype).cuda()
+    got = prefill(cache, q, 0, n, window=window, sinks=sinks).double().cpu()
+    ref = P.attention(q.double().cpu(), cache.k_rows[0].double(), cache.v_rows[0].double(), torch.arange(length - n, length),
+                      hd ** -0.5, window, sinks)
+    assert bool(((got - ref[0]).abs() <= bound(ref, length, dtype)).all())

@@ -8,9 +8,13 @@
 //   S = Q K^T       tcgen05.mma, both operands K-major in 128-byte-swizzled
 //                   shared tiles, S (f32) in TMEM
 //   P = 2^(S - m)   one thread per row: the row maximum and sum need no
-//                   exchange; P (16 bits) overwrites S in TMEM
-//   O += P V        tcgen05.mma with P from TMEM and V (rows of positions,
-//                   MN-major) from shared memory, O (f32) in TMEM
+//                   exchange; P overwrites S in TMEM, as a sum of two 16-bit
+//                   values (what the first leaves is rounded again), which keeps a
+//                   weight to 2^-17 (bf16), so that the output carries its own
+//                   rounding only
+//   O += P V        tcgen05.mma, a product for each part of P, with P from TMEM
+//                   and V (rows of positions, MN-major) from shared memory, O (f32)
+//                   in TMEM
 // The tiles A and B alternate on the tensor cores: while they work on one, the
 // softmax threads work on the other.  O is rescaled only when a row's maximum
 // has grown by more than 8 (a factor of 256, which both types hold), which after
@@ -25,13 +29,14 @@
 // whose boxes would break the swizzle, are gathered row by row with cp.async by
 // warps 9 to 11.
 //
-// Bound by the chain of one row tile, not by a pipe: softmax 1860 clocks (1024 of
-// them exponentials at the MUFU rate), then P V and the next Q K^T 1050 and the
-// hand-overs, 3440 per tile of 128 positions where the tensor cores need 2048 for
-// both row tiles.  Measured (32 / 8 heads x 128, bf16): 2048 tokens 51 us (0.67
-// PFLOP/s), 8192 under a window of 4096 437 to 456 us (0.93); 11 chunks of 1 to 511
-// (32 / 4 x 64, f16) 90 us.  P in columns of its own at 64 values, so that the next
-// Q K^T need not wait for P V, gave nothing (3370 clocks to 3570 to 3740).
+// Bound by the chain of one row tile, not by a pipe: the softmax with its 1024 clocks
+// of exponentials at the MUFU rate and the rounding of both parts of P, then P V (1024
+// clocks at 128 values) and the next Q K^T (512), and the hand-overs.  Measured (32 /
+// 8 heads x 128, bf16): 2048 tokens 64 us (0.53 PFLOP/s), 8192 under a window of 4096
+// 593 us (0.70); 11 chunks of 1 to 511 (32 / 4 x 64, f16) 115 us.  With P as one 16-bit
+// value it was 53, 459 and 96 us, at an error against 64 bits of 0.0020 (bf16) and
+// 2.9e-4 (f16) of the output in place of the 0.0016 and 2.1e-4 that the output's rounding
+// makes alone.
 //
 // The scale is taken positive (a negative one negates Q in the first product),
 // so the maximum of S is the maximum of the scaled scores.
@@ -371,8 +376,10 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
         const uint64_t v = dv + (kt & 1) * (C::TILE >> 4);
         if (elect_one()) {
 #pragma unroll
-          for (int kk = 0; kk < TN / 16; ++kk)
-            mma_f16_ts(256 + w * HD, w * TN + kk * 8, v + kk * 128, id_o, !(first && kk == 0));
+          for (int part = 1; part >= 0; --part)  // the low part of P, then the high one
+#pragma unroll
+            for (int kk = 0; kk < TN / 16; ++kk)
+              mma_f16_ts(256 + w * HD, w * TN + part * (TN / 2) + kk * 8, v + kk * 128, id_o, !(first && part == 1 && kk == 0));
         }
         __syncwarp();
       };
@@ -630,17 +637,26 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
         const f2 scale = pk(a.scale2, a.scale2), base = pk(b, b);
         f2 sum[2] = {pk(0.f, 0.f), pk(0.f, 0.f)};
 #pragma unroll
-        for (int i = 0; i < TN / 2; ++i) {
-          const f2 x = fma2(pk(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale, base);
-          float u, v;
-          unpk(x, u, v);
-          u = ex2(u);
-          v = ex2(v);
-          sum[i & 1] = add2(sum[i & 1], pk(u, v));
-          s[i] = pack2<T>(u, v);
-          if (i == TN / 4 - 1) tmem_st32(ts, s);
+        for (int h = 0; h < 2; ++h) {
+          uint32_t hi[TN / 4], lo[TN / 4];
+#pragma unroll
+          for (int i = 0; i < TN / 4; ++i) {
+            const int c = h * (TN / 2) + 2 * i;
+            const f2 x = fma2(pk(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), scale, base);
+            float u, v;
+            unpk(x, u, v);
+            u = ex2(u);
+            v = ex2(v);
+            const f2 p = pk(u, v);
+            sum[i & 1] = add2(sum[i & 1], p);
+            hi[i] = pack2<T>(u, v);
+            const float2 r = unpack2<T>(hi[i]);
+            unpk(sub2(p, pk(r.x, r.y)), u, v);
+            lo[i] = pack2<T>(u, v);
+          }
+          tmem_st32(ts + h * (TN / 4), hi);
+          tmem_st32(ts + TN / 2 + h * (TN / 4), lo);
         }
-        tmem_st32(ts + 32, s + 32);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
