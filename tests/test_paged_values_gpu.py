@@ -80,3 +80,40 @@ def test_prefill_keeps_the_weights_exact(dtype, hd, heads, n, length, window, si
     ref = P.attention(q.double().cpu(), cache.k_rows[0].double(), cache.v_rows[0].double(), torch.arange(length - n, length),
                       hd ** -0.5, window, sinks)
     assert bool(((got - ref[0]).abs() <= bound(ref, length, dtype)).all())
+
+
+# What a weight of an f16 cache is held to, as a share of the row's largest: f16 ends at steps of 2^-24, half a step
+# off at most, and weights are kept times 2^15 (decode) and 2^13 (prefill, whose running maximum may lag by 2 bits).
+F16_STEP = {"decode": 2.0 ** -40, "prefill": 2.0 ** -38}
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("nats", [12.0, 15.0, 18.0])
+@pytest.mark.parametrize("where", ["first", "middle"])
+def test_many_small_weights_beside_a_large_one(dtype, nats, where):
+    """One key far above all others, its value 0: the output is made of the small weights alone."""
+    length, hd, n = 20000, 64, 5
+    cache = P.Cache([length], 1, hd, 64, dtype, 77)
+    g = torch.Generator().manual_seed(10)
+    at = 0 if where == "first" else 11111
+    k = torch.zeros(length, 1, hd)
+    k[:, 0, 1:] = 0.02 * torch.randn(length, hd - 1, generator=g)  # the others differ a little
+    k[at, 0, 0] = nats
+    v = torch.rand(length, 1, hd, generator=g) + 0.5
+    v[at] = 0.0
+    cache.k_rows[0], cache.v_rows[0] = k.to(dtype), v.to(dtype)
+    t = torch.arange(length)
+    pg = cache.table[0].cpu().long()[t // 64].cuda()
+    cache.k[pg, :, (t % 64).cuda()] = cache.k_rows[0].cuda()
+    cache.v[pg, :, (t % 64).cuda()] = cache.v_rows[0].cuda()
+    q = torch.randn(n, 4, hd, generator=g)
+    q[:, :, 0] = 1.0
+    q = q.to(dtype).cuda()
+    pos = torch.arange(length - n, length)
+    ref = P.attention(q.double().cpu(), cache.k_rows[0].double(), cache.v_rows[0].double(), pos, 1.0)
+    for what, got in (("prefill", prefill(cache, q, 0, n, scale=1.0)), ("decode", decode(cache, q[-1:], scale=1.0))):
+        r = ref if what == "prefill" else tuple(x[-1:] for x in ref)
+        small = length * F16_STEP[what] * 1.5 if dtype == F16 else 0.0
+        err = (got.double().cpu() - r[0]).abs()
+        tol = bound(r, length, dtype, small)
+        assert bool((err <= tol).all()), f"{what}: {float((err / tol).max()):.2f} of the bound"

@@ -17,8 +17,8 @@
 //                   in TMEM
 // The tiles A and B alternate on the tensor cores: while they work on one, the
 // softmax threads work on the other.  O is rescaled only when a row's maximum
-// has grown by more than 8 (a factor of 256, which both types hold), which after
-// the first tiles hardly ever happens.
+// has grown by more than Range::LAG bits, which after the first tiles hardly ever
+// happens.
 //
 // Warps 0-3: softmax of A; 4-7: of B; 8: issues the MMAs; 10: brings Q, K and V
 // by TMA, K and V into two stages each, one box per page and 64 values (4-d map
@@ -204,6 +204,14 @@ template <typename T> __device__ __forceinline__ uint32_t nonfinite2(uint32_t w)
 }
 
 constexpr int TQ = 128, TN = 128, TC_THREADS = 384;
+// How far (in bits) the maximum that P is relative to may lag behind a row's own before O
+// is rescaled, and the power of two that P is kept times.  bf16 has f32's range.  f16
+// ends at steps of 2^-24, so weights far below the largest would be lost from the
+// products, but not from the row's sum: they are kept times 2^13 (2^15 at most, with
+// the lag), which holds them to 2^-38 of the largest.  4096 tokens on 4096 (32 / 8 heads
+// x 128): 522 us; lag 8 and 2^7 (2^-32) 516; no lag and 2^15 (2^-40) 548.
+template <typename T> struct Range { static constexpr float LAG = 8.f, UP = 0.f; };
+template <> struct Range<__half> { static constexpr float LAG = 2.f, UP = 13.f; };
 // Registers per thread after the split: softmax warps, MMA and gather warps.
 // setmaxnreg draws on what the CTA was launched with, so the sum of the shares
 // must not pass it (checked before the launch).
@@ -617,7 +625,7 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
 #pragma unroll
           for (int q = 0; q < 4; ++q) mx[q] = max3(mx[q], __uint_as_float(s[i + 2 * q]), __uint_as_float(s[i + 2 * q + 1]));
         const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale2;
-        if (__any_sync(0xffffffffu, top > m + 8.f)) {
+        if (__any_sync(0xffffffffu, top > m + Range<T>::LAG)) {
           const float mn = fmaxf(m, top), f2o = m == -INFINITY ? 0.f : ex2(m - mn);
           m = mn;
           l *= f2o;
@@ -633,7 +641,7 @@ paged_prefill_tc_kernel(const __grid_constant__ AttnArgs a, const __grid_constan
             }
           }
         }
-        const float b = m == -INFINITY ? 0.f : -m;
+        const float b = m == -INFINITY ? 0.f : Range<T>::UP - m;
         const f2 scale = pk(a.scale2, a.scale2), base = pk(b, b);
         f2 sum[2] = {pk(0.f, 0.f), pk(0.f, 0.f)};
 #pragma unroll
