@@ -39,6 +39,14 @@ def decode(cache, q, **kw):
     return got
 
 
+def decode_all(cache, q, s, **kw):
+    """Every row of q as the new token of sequence s."""
+    n = q.shape[0]
+    got = ops.paged_attention_decode(q, cache.k, cache.v, cache.table[s:s + 1].repeat(n, 1), cache.d_lens[s:s + 1].repeat(n), **kw)
+    ops.check_device_error()
+    return got
+
+
 def prefill(cache, q, s, n, **kw):
     """The last n tokens of sequence s alone."""
     got = ops.paged_attention_prefill(q, cache.k, cache.v, cache.table[s:s + 1], cache.d_lens[s:s + 1], i32(0, n), **kw)
@@ -117,3 +125,28 @@ def test_many_small_weights_beside_a_large_one(dtype, nats, where):
         err = (got.double().cpu() - r[0]).abs()
         tol = bound(r, length, dtype, small)
         assert bool((err <= tol).all()), f"{what}: {float((err / tol).max()):.2f} of the bound"
+
+
+def test_decode_small_weights_within_a_warp():
+    """As above where a warp walks its positions alone: more sequences (of one prompt's pages) than CTAs."""
+    length, hd, n = 1000, 64, 320
+    cache = P.Cache([length], 2, hd, 64, F16, 79)
+    g = torch.Generator().manual_seed(12)
+    k = torch.zeros(length, 2, hd)
+    k[:, :, 1:] = 0.02 * torch.randn(length, 2, hd - 1, generator=g)
+    k[3, :, 0] = 18.0
+    v = torch.rand(length, 2, hd, generator=g) + 0.5
+    v[3] = 0.0
+    cache.k_rows[0], cache.v_rows[0] = k.to(F16), v.to(F16)
+    t = torch.arange(length)
+    pg = cache.table[0].cpu().long()[t // 64].cuda()
+    cache.k[pg, :, (t % 64).cuda()] = cache.k_rows[0].cuda()
+    cache.v[pg, :, (t % 64).cuda()] = cache.v_rows[0].cuda()
+    q = torch.randn(n, 8, hd, generator=g)
+    q[:, :, 0] = 1.0
+    q = q.to(F16).cuda()
+    got = ops.paged_attention_decode(q, cache.k, cache.v, cache.table.repeat(n, 1), cache.d_lens.repeat(n), scale=1.0)
+    ops.check_device_error()
+    ref = P.attention(q.double().cpu(), cache.k_rows[0].double(), cache.v_rows[0].double(), torch.full((n,), length - 1), 1.0)
+    err, tol = (got.double().cpu() - ref[0]).abs(), bound(ref, length, F16, length * F16_STEP["decode"] * 1.5)
+    assert bool((err <= tol).all()), f"{float((err / tol).max()):.2f} of the bound"

@@ -10,6 +10,8 @@
 // legacy tensor path gives at HBM rate, so mma.sync (whose operands need no
 // TMEM round trip) is enough here.
 #pragma once
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace vtb {
@@ -141,9 +143,12 @@ template <typename T, int HD, int NT, bool F32 = Elem<T>::f32> struct Step;
 // 16-bit types: m16n8k16 with ldmatrix; rows of HD values with their 16-byte
 // pieces swizzled by the row (piece ^ row % 8), so ldmatrix is conflict-free.
 // P enters the second product as a sum of two 16-bit values, which keeps it
-// exact to 2^-17 (bf16): the output then carries its own rounding only.
+// exact to 2^-17 (bf16): the output then carries its own rounding only.  f16 ends at
+// steps of 2^-24: P is kept times 2^15, which holds weights to 2^-40 of the largest
+// (they would be lost from the products, but not from the sum).
 template <typename T, int HD, int NT> struct Step<T, HD, NT, false> {
   static constexpr bool F = false;
+  static constexpr int UP = std::is_same<T, __half>::value ? 15 : 0;
   static constexpr int PIECES = HD / 8, ROW = HD * 2;  // 16-byte pieces and bytes of a staged row
   static constexpr int QREGS = HD / 8;
   uint32_t q[NT][QREGS];
@@ -217,6 +222,7 @@ template <typename T, int HD, int NT> struct Step<T, HD, NT, false> {
 // pieces are swizzled by the row so that these fall into different banks.
 template <int HD, int NT> struct Step<float, HD, NT, true> {
   static constexpr bool F = true;
+  static constexpr int UP = 0;
   static constexpr int PIECES = HD / 4, ROW = HD * 4;
   static constexpr int QREGS = HD / 4;
   float q[NT][QREGS];
@@ -326,8 +332,9 @@ template <int HD, int NT> struct Step<float, HD, NT, true> {
 // Online softmax of the warp's 16 scores per vector (in units of log2): m is
 // the running maximum, l this lane's share of the running sum.  A row whose
 // maximum is still -inf keeps p = 0.  On return s holds p, f the factors that
-// o needs (all 1 unless the result is true, the same for the whole warp).
-template <int NT>
+// o needs (all 1 unless the result is true, the same for the whole warp).  p and l
+// are kept times 2^UP.
+template <int NT, int UP>
 __device__ __forceinline__ bool softmax_step(float (&s)[NT][4], float (&m)[NT][2], float (&l)[NT][2], float (&f)[NT][2]) {
   bool moved = false;
 #pragma unroll
@@ -337,8 +344,8 @@ __device__ __forceinline__ bool softmax_step(float (&s)[NT][4], float (&m)[NT][2
       float x = fmaxf(s[nt][c], s[nt][c + 2]);
 #pragma unroll
       for (int off = 4; off < 32; off <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, off));
-      const float mn = fmaxf(m[nt][c], x), base = mn == -INFINITY ? 0.f : mn;
-      f[nt][c] = exp2f(m[nt][c] - base);
+      const float mn = fmaxf(m[nt][c], x), base = mn == -INFINITY ? 0.f : mn - UP;
+      f[nt][c] = exp2f(m[nt][c] - (mn == -INFINITY ? 0.f : mn));
       moved |= mn != m[nt][c];
       m[nt][c] = mn;
       s[nt][c] = exp2f(s[nt][c] - base);

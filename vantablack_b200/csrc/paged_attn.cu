@@ -266,7 +266,7 @@ paged_decode_kernel(const __grid_constant__ AttnArgs a, int hgroups) {
         s[nt][3] = in1 ? s[nt][3] * a.scale2 : -INFINITY;
       }
       float f[NT][2];
-      const bool moved = softmax_step<NT>(s, m, l, f);
+      const bool moved = softmax_step<NT, S::UP>(s, m, l, f);
       st.pv(vb, lane, s, f, moved, o);
     }
     if (cur.t + 1 < cur.nt && i + 1 < n) {
