@@ -54,6 +54,119 @@ def prefill(cache, q, s, n, **kw):
     return got
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd,heads", [(64, 8), (128, 8), (64, 24), (128, 40)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (70, 5)])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_decode_infinities_and_nans_of_v_reach_their_values_only(dtype, hd, heads, window, sinks, value):
+    """As in prefill: a query that sees a V row with such a value gets it there; every other value is as if it were 0.
+    The sequences lie within one CTA, and over many."""
+    cache = P.Cache([250, 40, 9001, 1], 2, hd, 16, dtype, 71)
+    bad = {0: [2, 45, 249], 2: [3, 4000, 8999], 3: [0]}
+    for s, at in bad.items():
+        for t in at:
+            put(cache, "v", s, t, 1, 5, value)
+    q = torch.randn(4, heads, hd, generator=torch.Generator().manual_seed(4)).to(dtype).cuda()
+    got = decode(cache, q, window=window, sinks=sinks).double().cpu()
+    for s, at in bad.items():
+        n = cache.lens[s]
+        see = P.visible(torch.tensor([n - 1]), torch.tensor(at), window, sinks)
+        assert bool(see.any())
+        for t in at:
+            cache.v_rows[s][t, 1, 5] = 0.0
+        ref = P.attention(q[s:s + 1].double().cpu(), cache.k_rows[s].double(), cache.v_rows[s].double(), torch.tensor([n - 1]),
+                          hd ** -0.5, window, sinks)
+        ok = (got[s:s + 1] - ref[0]).abs() <= bound(ref, n, dtype)
+        hit = got[s, heads // 2:, 5]  # kv head 1's queries
+        assert bool(torch.isnan(hit).all()) if math.isnan(value) else bool((hit == value).all())
+        ok[:, heads // 2:, 5] = True
+        assert bool(ok.all())
+    assert bool(torch.isfinite(got[1]).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_infinities_of_both_signs_make_nan(dtype):
+    cache = P.Cache([300], 2, 64, 16, dtype, 72)
+    put(cache, "v", 0, 20, 0, 7, math.inf)
+    put(cache, "v", 0, 200, 0, 7, -math.inf)
+    q = torch.randn(30, 8, 64, generator=torch.Generator().manual_seed(5)).to(dtype).cuda()
+    for got in (decode(cache, q[-1:]), prefill(cache, q, 0, 30)):
+        bad = ~torch.isfinite(got)
+        assert bool(torch.isnan(got[:, :4, 7]).all())
+        bad[:, :4, 7] = False
+        assert not bool(bad.any())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("scale", [0.125, -0.2])
+@pytest.mark.parametrize("what", ["decode"])
+def test_infinities_of_k(dtype, hd, scale, what):
+    """A score of -inf has the weight 0: the query is as if it did not see the position.  A score of inf gives NaN.
+    Positions in tiles that all rows see, at the edge, and in the rest of the cache."""
+    cache = P.Cache([700, 33], 2, hd, 16, dtype, 73)
+    at = [5, 300, 655]
+    for t in at:
+        put(cache, "k", 0, t, 1, 3, math.inf)
+    n = 60 if what == "prefill" else 6
+    q = torch.randn(n, 6, hd, generator=torch.Generator().manual_seed(6)).to(dtype)
+    q[:, :, 3] = q[:, :, 3].abs().clamp(min=0.1) * torch.where(torch.arange(n) % 3 == 0, 1.0, -1.0).to(dtype)[:, None]
+    q = q.cuda()
+    if what == "prefill":
+        rows, pos = prefill(cache, q, 0, n, scale=scale).double().cpu(), torch.arange(640, 700)
+    else:
+        rows, pos = decode_all(cache, q, 0, scale=scale).double().cpu(), torch.full((n,), 699)
+    qq = q.double().cpu()
+    up = (qq[:, 0, 3] * scale > 0)  # the score of such a position is +inf
+    assert bool(up.any()) and not bool(up.all())
+    assert bool(torch.isnan(rows[up][:, 3:]).all())
+    # the others: what is left of the cache without these positions
+    keep = torch.tensor([t for t in range(700) if t not in at])
+    for r in torch.nonzero(~up).flatten().tolist():
+        t = keep[keep <= pos[r]]
+        k, v = cache.k_rows[0].double()[t, 1:], cache.v_rows[0].double()[t, 1:]
+        ref = P.attention(qq[r:r + 1, 3:], k, v, torch.tensor([len(t) - 1]), scale)
+        assert bool(((rows[r:r + 1, 3:] - ref[0]).abs() <= bound(ref, 700, dtype)).all()), r
+    ref = P.attention(qq[:, :3], cache.k_rows[0].double()[:, :1], cache.v_rows[0].double()[:, :1], pos, scale)
+    assert bool(((rows[:, :3] - ref[0]).abs() <= bound(ref, 700, dtype)).all())  # kv head 0 has none
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("huge", [F32_MAX, -F32_MAX, 3.4027e38, 1e38])
+@pytest.mark.parametrize("what", ["decode"])
+def test_f32_values_at_the_end_of_the_range(hd, huge, what):
+    """Finite values whose leading part would round to infinity.  V: hidden ones stay hidden, seen ones count with their
+    weight.  K: a query that is 0 there is as if they were, one that is not (a score of -1e7) as if it did not see them."""
+    cache = P.Cache([400, 90], 2, hd, 16, F32, 74)
+    for t in (10, 390):
+        put(cache, "v", 0, t, 1, 9, huge)
+    for t in (30, 395):
+        put(cache, "k", 0, t, 0, 2, huge)
+    for head in range(2):  # the largest weight is another position's: sums of the huge values stay in range
+        put(cache, "k", 0, 1, head, 0, 90.0)
+    n = 50 if what == "prefill" else 4
+    q = torch.randn(n, 8, hd, generator=torch.Generator().manual_seed(7))
+    q[:, :, 0] = 1.0
+    q[:, :, 2] = torch.where(torch.arange(n) % 2 == 0, 0.0, -1e-30 * (1 if huge > 0 else -1))[:, None]
+    q = q.cuda()
+    if what == "prefill":
+        rows, pos = prefill(cache, q, 0, n).double().cpu(), torch.arange(350, 400)
+    else:
+        rows, pos = decode_all(cache, q, 0).double().cpu(), torch.full((n,), 399)
+    qq = q.double().cpu()
+    assert bool(torch.isfinite(rows).all())
+    k, v = cache.k_rows[0].double(), cache.v_rows[0].double()
+    for r in range(n):
+        t = torch.arange(int(pos[r]) + 1)
+        if qq[r, 0, 2] != 0:
+            t = t[(t != 30) & (t != 395)]
+        got = rows[r:r + 1] if qq[r, 0, 2] == 0 else rows[r:r + 1, :4]  # (kv head 0's queries)
+        ref = P.attention(qq[r:r + 1, :got.shape[1]], k[t, :2 if got.shape[1] == 8 else 1], v[t, :2 if got.shape[1] == 8 else 1],
+                          torch.tensor([len(t) - 1]), hd ** -0.5)
+        # a leading part cut off instead of rounded: 2^-19 of the terms in place of 2^-20
+        assert bool(((got - ref[0]).abs() <= bound(ref, 400, F32) + ref[1] * 2.0 ** -19).all()), r
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("dtype", [F16, BF16])
 @pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan])

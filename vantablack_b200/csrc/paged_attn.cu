@@ -42,6 +42,10 @@ __device__ __forceinline__ Span span_of(int p0, int p1, int window, int sinks) {
   return s;
 }
 
+// Factors between maxima are not let down to 0, so that an infinity stays one in parts
+// that weigh nothing (finite parts of them stay below anything that counts).
+constexpr float TINY = 1.2e-38f;
+
 // ======================= decode =======================
 // HBM bound: K and V are read once.  The visible positions of every (sequence,
 // kv head) are cut into tiles of 16 per warp, all tiles put in one line, and the line
@@ -133,6 +137,67 @@ template <int TILE> struct LineCursor {  // one tile of the line
     while (s < a.kv.n_seqs && (enter(a), nt == 0));
   }
 };
+
+// One query vector's share of a warp (its 16 positions of tiles t0 ... t1) once more, in
+// plain f32.  The tensor cores get P, and in f32 every operand, in two parts, where
+// an infinity becomes NaN (inf * 0, inf - inf) and a finite value next to the end of
+// f32's range rounds to infinity.  Either leaves a sum that is not finite, so the fast
+// path looks at nothing but its sums at the end of a share.  Here scores of -inf
+// have the weight 0, and infinities and NaN of V reach their value whatever the
+// weight (as in prefill).  One infinity in 131072 positions (32 / 8 heads x 128, bf16):
+// 0.1 -> 0.36 ms; V of NaN throughout 3.0 ms.  out: HD sums in shared memory;
+// returns (max, sum).
+template <typename T, int HD, int TILE, int UP>
+__device__ __noinline__ float2 decode_again(const AttnArgs& a, const T* q, int s, int kvh, Span sp, int t0, int t1, float* out) {
+  constexpr int PER = HD / 32;  // values per lane
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  float x[PER], o[PER] = {}, m = -INFINITY, l = 0.f;
+#pragma unroll
+  for (int k = 0; k < PER; ++k) x[k] = to_f(q[lane * PER + k]);
+  for (int t = t0; t <= t1; ++t) {
+    const int base = t * TILE + warp * 16, n = min(16, sp.n - base);
+    if (n <= 0) break;
+    long long off = 0;  // lanes i and i + 16: row i
+    float score = -INFINITY;
+    if ((lane & 15) < n) {
+      const int pos = sp.pos(base + (lane & 15));
+      off = page_row(a.kv, a.kv.table[s * a.kv.table_stride + (pos >> a.kv.page_shift)], pos) + kvh * a.kv.head_stride;
+    }
+    for (int i = 0; i < n; ++i) {
+      const T* k = reinterpret_cast<const T*>(a.kv.k + __shfl_sync(0xffffffffu, off, i)) + lane * PER;
+      float d = 0.f;
+#pragma unroll
+      for (int j = 0; j < PER; ++j) d = fmaf(x[j], to_f(k[j]), d);
+      d = warp_sum(d);
+      if ((lane & 15) == i) score = d * a.scale2;
+    }
+    float top = score;
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const float mn = fmaxf(m, top), b = mn == -INFINITY ? 0.f : mn, f = fmaxf(exp2f(m - b), TINY);
+    const float p = exp2f(score - (b - UP));
+    float sum = p;
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    l = l * f + sum;
+    m = mn;
+    float add[PER] = {};
+    for (int i = 0; i < n; ++i) {
+      const T* v = reinterpret_cast<const T*>(a.kv.v + __shfl_sync(0xffffffffu, off, i)) + lane * PER;
+      const float w = __shfl_sync(0xffffffffu, p, i);
+#pragma unroll
+      for (int j = 0; j < PER; ++j) {
+        const float y = to_f(v[j]);
+        add[j] = fabsf(y) < INFINITY ? fmaf(w, y, add[j]) : add[j] + y;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < PER; ++j) o[j] = o[j] * f + add[j];
+  }
+#pragma unroll
+  for (int k = 0; k < PER; ++k) out[lane * PER + k] = o[k];
+  return make_float2(m, l);
+}
 
 template <typename T, int HD, int NT>
 __global__ void __launch_bounds__(DecodeCfg<T, HD, NT>::WARPS * 32, Elem<T>::f32 ? 1 : 2)
@@ -286,6 +351,8 @@ paged_decode_kernel(const __grid_constant__ AttnArgs a, int hgroups) {
         *todo = make_int4(seq, cur.u, parts, first_part ? 0 : 1);
       }
     }
+    const Span sp = cur.sp;
+    const int t1 = cur.t, t0 = max(0, cur.t - i);  // the share's tiles
     cur.next(a, units);
     if (i + 1 < n) queries(cur.s, cur.u);  // on their way while the warps are joined
     float* slot = a.part + (2ll * blockIdx.x + (first_part ? 0 : 1)) * C::SLOT;
@@ -295,6 +362,30 @@ paged_decode_kernel(const __grid_constant__ AttnArgs a, int hgroups) {
       for (int c = 0; c < 2; ++c) {
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], off);
+        float zero = 0.f;  // 0 if the sums of vector 2t + c are finite, NaN otherwise
+#pragma unroll
+        for (int j = 0; j < HD / 16; ++j) zero = fmaf(o[nt][j][c], 0.f, fmaf(o[nt][j][c + 2], 0.f, zero));
+        // (16-bit scores are right as they are: a NaN among them is NaN here too)
+        const unsigned odd = __ballot_sync(0xffffffffu, zero != 0.f && (S::F || l[nt][c] == l[nt][c]));
+#pragma unroll 1
+        for (int v = 0; odd && v < 4; ++v) {
+          const int h = h0 + 8 * nt + 2 * v + c;
+          if (!(odd >> v & 0x11111111u) || h >= a.group) continue;
+          float* again = red + warp * 4 * (HD + 4);
+          const T* q = static_cast<const T*>(a.q) + seq * a.q_row + (long long)(kvh * a.group + h) * a.q_head;
+          const float2 now = decode_again<T, HD, C::TILE, S::UP>(a, q, seq, kvh, sp, t0, t1, again);
+          __syncwarp();
+          if (t == v) {
+            m[nt][c] = now.x;
+            l[nt][c] = now.y;
+#pragma unroll
+            for (int j = 0; j < HD / 16; ++j) {
+              o[nt][j][c] = again[S::dim(j, 0, g)];
+              o[nt][j][c + 2] = again[S::dim(j, 1, g)];
+            }
+          }
+          __syncwarp();
+        }
         if (g == 0) ml[warp * 8 + 2 * t + c] = make_float2(m[nt][c], l[nt][c]);
       }
       __syncthreads();
@@ -303,7 +394,7 @@ paged_decode_kernel(const __grid_constant__ AttnArgs a, int hgroups) {
       for (int c = 0; c < 2; ++c) {
         float M = -INFINITY;
         for (int w = 0; w < C::WARPS; ++w) M = fmaxf(M, ml[w * 8 + 2 * t + c].x);
-        f[c] = exp2f(m[nt][c] - (M == -INFINITY ? 0.f : M));
+        f[c] = fmaxf(exp2f(m[nt][c] - (M == -INFINITY ? 0.f : M)), TINY);
       }
 #pragma unroll
       for (int v0 = 0; v0 < 8; v0 += 4) {  // vectors v0 ... v0 + 3 of the eight
@@ -385,7 +476,7 @@ __global__ void __launch_bounds__(HD) paged_decode_join_kernel(const __grid_cons
   const float b = M == -INFINITY ? 0.f : M;
   float L = 0.f;
   for (int i = d; i < n; i += HD) {
-    const float e = exp2f(weight[i] - b);
+    const float e = fmaxf(exp2f(weight[i] - b), TINY);
     weight[i] = e;
     L += slot(i)[NT * 8 + h] * e;
   }

@@ -800,7 +800,7 @@ __global__ void __launch_bounds__(256) paged_prefill_join_kernel(const __grid_co
 #pragma unroll 4
     for (int i = 0; i < splits; ++i) {
       const float* q = p + (long long)i * SLOT;
-      const float e = fmaxf(exp2f(q[r] - b), 1.2e-38f);  // not 0, for the infinities of a split that weighs nothing
+      const float e = fmaxf(exp2f(q[r] - b), TINY);
       L += q[ROWS + r] * e;
 #pragma unroll
       for (int k = 0; k < V; k += 4) {
