@@ -100,7 +100,7 @@ def test_infinities_of_both_signs_make_nan(dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("scale", [0.125, -0.2])
-@pytest.mark.parametrize("what", ["decode"])
+@pytest.mark.parametrize("what", ["decode", "prefill"])
 def test_infinities_of_k(dtype, hd, scale, what):
     """A score of -inf has the weight 0: the query is as if it did not see the position.  A score of inf gives NaN.
     Positions in tiles that all rows see, at the edge, and in the rest of the cache."""

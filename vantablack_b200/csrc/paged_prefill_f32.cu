@@ -54,6 +54,30 @@ struct F32Bars {
   int bad0, bad1;  // tiles with infinities or NaN in V lie in [bad0, bad1) (add_nonfinite)
 };
 
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN if one is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// The row's scores once more where they are NaN, from the cache in plain f32: an
+// infinity in K or Q, or a finite value next to the end of f32's range, has no second
+// part that adds up with the first (inf - inf), and a score of -inf has to weigh
+// nothing.  x: the tile's scores, from index i0 of the span on.
+template <int HD>
+__device__ __noinline__ void scores_again(const AttnArgs& a, const float* q, int s, int kvh, const Span& sp, int i0, float* x) {
+  for (int i = 0; i < FN; ++i) {
+    if (!isnan(x[i])) continue;
+    const int t = sp.pos(i0 + i);
+    const char* k = a.kv.k + page_row(a.kv, __ldg(a.kv.table + s * a.kv.table_stride + (t >> a.kv.page_shift)), t) + kvh * a.kv.head_stride;
+    float d = 0.f;
+    for (int c = 0; c < HD; c += 4) {
+      const float4 u = *reinterpret_cast<const float4*>(q + c), v = *reinterpret_cast<const float4*>(k + c * 4);
+      d = fmaf(u.x, v.x, d); d = fmaf(u.y, v.y, d); d = fmaf(u.z, v.z, d); d = fmaf(u.w, v.w, d);
+    }
+    x[i] = a.negate ? -d : d;
+  }
+}
+
 template <int HD>
 __global__ void __launch_bounds__(F_THREADS, 1) paged_prefill_f32_kernel(const __grid_constant__ AttnArgs a, int splits) {
   using C = F32Prefill<HD>;
@@ -329,12 +353,32 @@ __global__ void __launch_bounds__(F_THREADS, 1) paged_prefill_f32_kernel(const _
             if (!(see >> i & 1)) s[c + i] = 0xff800000u;
         }
       }
-      float mx[2] = {-INFINITY, -INFINITY};
+      auto largest = [&]() {  // NaN if a score that is seen is NaN
+        float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < FN; i += 4)
+        for (int i = 0; i < FN; i += 4)
 #pragma unroll
-        for (int q = 0; q < 2; ++q) mx[q] = max3(mx[q], __uint_as_float(s[i + 2 * q]), __uint_as_float(s[i + 2 * q + 1]));
-      const float mn = fmaxf(m, fmaxf(mx[0], mx[1]) * a.scale2), b = mn == -INFINITY ? 0.f : mn;
+          for (int q = 0; q < 2; ++q) mx[q] = max3_nan(mx[q], __uint_as_float(s[i + 2 * q]), __uint_as_float(s[i + 2 * q + 1]));
+        return max3_nan(mx[0], mx[1], mx[0]);
+      };
+      float top = largest();
+      int again = __any_sync(0xffffffffu, row && isnan(top));
+      asm volatile("" : "+r"(again));
+#pragma unroll 1
+      for (; again > 0; --again) {
+        float x[FN];
+#pragma unroll
+        for (int i = 0; i < FN; ++i) x[i] = __uint_as_float(s[i]);
+        if (row) {
+          const int t = a.token(r);
+          const float* q = static_cast<const float*>(a.q) + (rt.r0 + tok0 + t) * a.q_row + (long long)(kvh * a.group + r - t * a.group) * a.q_head;
+          scores_again<HD>(a, q, rt.s, kvh, sp, v0, x);
+        }
+#pragma unroll
+        for (int i = 0; i < FN; ++i) s[i] = __float_as_uint(x[i]);
+        top = largest();
+      }
+      const float mn = fmaxf(m, top * a.scale2), b = mn == -INFINITY ? 0.f : mn;
       f = ex2(m - b);
       m = mn;
       float sum[2] = {0.f, 0.f};
