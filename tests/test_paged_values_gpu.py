@@ -133,7 +133,7 @@ def test_infinities_of_k(dtype, hd, scale, what):
 
 @pytest.mark.parametrize("hd", [64, 128])
 @pytest.mark.parametrize("huge", [F32_MAX, -F32_MAX, 3.4027e38, 1e38])
-@pytest.mark.parametrize("what", ["decode"])
+@pytest.mark.parametrize("what", ["decode", "prefill"])
 def test_f32_values_at_the_end_of_the_range(hd, huge, what):
     """Finite values whose leading part would round to infinity.  V: hidden ones stay hidden, seen ones count with their
     weight.  K: a query that is 0 there is as if they were, one that is not (a score of -1e7) as if it did not see them."""

@@ -123,8 +123,10 @@ __device__ __forceinline__ void mma_tf32(float* c, const uint32_t* a, uint32_t b
 // x = hi + lo with both in tf32 (11 significant bits): hi rounded to nearest,
 // so lo's sign is free and cutting it to 11 bits (relative 2^-21 of x at most)
 // has no bias.  A product of two split values drops lo * lo, 2^-22 relative.
-__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
-  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+// (half = 0 cuts hi off instead, 2 bits worse in all: for finite values from 0x7f7ff000
+// on, which would round to infinity.)
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo, uint32_t half = 0x1000u) {
+  hi = (__float_as_uint(x) + half) & 0xffffe000u;
   lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
 }
 

@@ -236,14 +236,22 @@ __global__ void __launch_bounds__(F_THREADS, 1) paged_prefill_f32_kernel(const _
       for (int j = 0; j < n; ++j) {
         if (j) ok = warp_wait(&bar.v_freed, (j - 1) & 1);
         if (!ok) break;
-        bool odd = false;
+        bool odd = false;  // values that have no hi and lo: infinities, NaN, and what would round to infinity
 #pragma unroll
-        for (int i = 0; i < POS; ++i) odd |= (__float_as_uint(x[i]) & 0x7f800000u) == 0x7f800000u;
+        for (int i = 0; i < POS; ++i) odd |= (__float_as_uint(x[i]) & 0x7fffffffu) >= 0x7f7ff000u;
+        uint32_t half = 0x1000u;
         if (__any_sync(0xffffffffu, odd)) {
+          bool bad = false, huge = false;
 #pragma unroll
           for (int i = 0; i < POS; ++i)
-            if ((__float_as_uint(x[i]) & 0x7f800000u) == 0x7f800000u) x[i] = 0.f;
-          if (lane == 0) {
+            if ((__float_as_uint(x[i]) & 0x7f800000u) == 0x7f800000u) {
+              x[i] = 0.f;
+              bad = true;
+            } else {
+              huge |= (__float_as_uint(x[i]) & 0x7fffffffu) >= 0x7f7ff000u;
+            }
+          if (huge) half = 0;
+          if (__any_sync(0xffffffffu, bad) && lane == 0) {
             atomicMin(&bar.bad0, j);
             atomicMax(&bar.bad1, j + 1);
           }
@@ -256,7 +264,7 @@ __global__ void __launch_bounds__(F_THREADS, 1) paged_prefill_f32_kernel(const _
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const float v = (j0 + j) * FN + p0 + i + c < sp.n ? x[i + c] : 0.f;
-            split_tf32(v, hi[c], lo[c]);
+            split_tf32(v, hi[c], lo[c], half);
           }
           st4(at, hi);
           st4(at + C::KV, lo);
