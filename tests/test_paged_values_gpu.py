@@ -263,3 +263,33 @@ def test_decode_small_weights_within_a_warp():
     ref = P.attention(q.double().cpu(), cache.k_rows[0].double(), cache.v_rows[0].double(), torch.full((n,), length - 1), 1.0)
     err, tol = (got.double().cpu() - ref[0]).abs(), bound(ref, length, F16, length * F16_STEP["decode"] * 1.5)
     assert bool((err <= tol).all()), f"{float((err / tol).max()):.2f} of the bound"
+
+
+def test_infinities_at_both_ends_of_a_long_context():
+    """f32: two bad V rows far apart cost a look at the rows between them, not a walk of every row's thread."""
+    length, n = 8704, 512
+    cache = P.Cache([length], 8, 128, 64, F32, 78)
+    q = torch.randn(n, 32, 128, generator=torch.Generator().manual_seed(11)).cuda()
+    starts = i32(0, n)
+
+    def time():
+        best = math.inf
+        for _ in range(4):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            torch.cuda.synchronize()
+            a.record()
+            got = ops.paged_attention_prefill(q, cache.k, cache.v, cache.table, cache.d_lens, starts)
+            b.record()
+            torch.cuda.synchronize()
+            best = min(best, a.elapsed_time(b))
+        ops.check_device_error()
+        return best, got
+
+    clean, want = time()
+    put(cache, "v", 0, 1, 1, 5, math.inf)
+    put(cache, "v", 0, length - n, 1, 6, -math.inf)
+    slow, got = time()
+    assert bool((got[:, 4:8, 5] == math.inf).all() and (got[:, 4:8, 6] == -math.inf).all())
+    got[:, 4:8, 5:7] = want[:, 4:8, 5:7]
+    assert torch.equal(got, want)
+    assert slow <= 10 * clean, f"{slow:.3f} ms, {clean:.3f} without"

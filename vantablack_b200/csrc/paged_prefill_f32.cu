@@ -51,7 +51,7 @@ template <int HD> struct F32Prefill {
 struct F32Bars {
   uint64_t q_full, k_full, k_freed, v_full, v_freed, s_full, p_full, o_full;
   uint32_t tmem;
-  int bad0, bad1;  // tiles with infinities or NaN in V lie in [bad0, bad1) (add_nonfinite)
+  int bad0, bad1;  // tiles with infinities or NaN in V lie in [bad0, bad1) (take_nonfinite)
 };
 
 __device__ __forceinline__ float max3_nan(float a, float b, float c) {  // NaN if one is
@@ -417,14 +417,19 @@ __global__ void __launch_bounds__(F_THREADS, 1) paged_prefill_f32_kernel(const _
     if (ok) {
       float* part = a.part + (long long)blockIdx.x * C::SLOT;
       const int bad0 = *reinterpret_cast<volatile int*>(&bar.bad0), bad1 = *reinterpret_cast<volatile int*>(&bar.bad1);
-      if (bad0 < bad1 && row) {
-        float x[HD];
+      if (bad0 < bad1) {
+        RowSums<HD> x;
 #pragma unroll
-        for (int i = 0; i < HD; ++i) x[i] = o[i];
-        for (int i = (j0 + bad0) * FN; i < min((j0 + bad1) * FN, vc); ++i)
-          if (i < va || i >= vb) add_nonfinite<float, HD>(a, rt.s, kvh, sp.pos(i), 0, x);
+        for (int i = 0; i < HD; ++i) x.o[i] = o[i];
+        for (uint32_t& y : x.set) y = 0;
+        x.done = row ? 0u : ~0u;
+        const int p = rt.ctx + tok0 + a.token(r), pa = a.window ? a.sinks : 0, pb = a.window ? p + 1 - a.window : 0;
+        // the tiles' positions: sinks, then what lies behind w0
+        const int i0 = (j0 + bad0) * FN, i1 = min((j0 + bad1) * FN, sp.n), behind = sp.w0 - sp.ns;
+        take_nonfinite<float, HD>(a, rt.s, kvh, i0, min(i1, sp.ns), sp.w0, pa, pb, p + 1, x);
+        take_nonfinite<float, HD>(a, rt.s, kvh, max(i0, sp.ns) + behind, i1 + behind, sp.w0, pa, pb, p + 1, x);
 #pragma unroll
-        for (int i = 0; i < HD; ++i) o[i] = x[i];
+        for (int i = 0; i < HD; ++i) o[i] = x.o[i];
       }
       const float inv = splits > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
       __syncwarp();

@@ -183,20 +183,6 @@ __device__ __noinline__ void take_nonfinite(const AttnArgs& a, int s, int kvh, i
     }
   }
 }
-// Adds the infinite and NaN ones of values [d0, d0 + N) of V at position t to o.
-template <typename T, int N>
-__device__ __noinline__ void add_nonfinite(const AttnArgs& a, int s, int kvh, int t, int d0, float* o) {
-  const int page = __ldg(a.kv.table + s * a.kv.table_stride + (t >> a.kv.page_shift));
-  const T* v = reinterpret_cast<const T*>(a.kv.v + page_row(a.kv, page, t) + kvh * a.kv.head_stride) + d0;
-  constexpr int PER = 16 / sizeof(T);
-  for (int d = 0; d < N; d += PER) {
-    float x[PER];
-    load_vec<T, T>(v + d, x);
-#pragma unroll
-    for (int k = 0; k < PER; ++k)
-      if ((__float_as_uint(x[k]) & 0x7f800000u) == 0x7f800000u) o[d + k] += x[k];
-  }
-}
 // Whether one of the 16-bit values in w is infinite or NaN, in bits 15 and 31 of the result.
 template <typename T> __device__ __forceinline__ uint32_t nonfinite2(uint32_t w) {
   constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
