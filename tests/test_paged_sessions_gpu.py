@@ -1,9 +1,10 @@
-"""Sessions on a paged state: a windowed prompt behind queued work, prompts in chunks under a window, head_dim 128."""
+"""Sessions on a paged state: a windowed prompt behind queued work, prompts in chunks under a window, head_dim 128,
+and calls that are refused in the middle of a token."""
 import numpy as np
 import pytest
 
 import oracle as O
-from vantablack_b200 import ops, synth as S
+from vantablack_b200 import _lib, ops, synth as S
 from vantablack_b200.model import Context, CudaModel, CudaState, HostWeights, LlamaConfig, PagedConfig
 
 pytestmark = pytest.mark.gpu
@@ -88,3 +89,26 @@ def test_head_dim_128_against_the_oracle():
         assert near(b[0], a, LOGITS) and y[0] == O.argmax(a)
     ops.check_device_error()
     m.close()
+
+
+def test_refused_calls_leave_a_begun_token(model):
+    """A prefill that finds no page, or holds a bad token, changes nothing: the token that was begun goes on."""
+    pc = PagedConfig(6, 16)
+    st, want = CudaState(model, 2, 64, paged=pc), CudaState(model, 2, 64, paged=pc)
+    t = tokens(60, 4)
+    for s in (st, want):
+        s.prefill(t[:20], 0)
+        s.prefill(t[:33], 1)
+    la, aa = want.step([7, 8], graph=False)
+    assert begin(st, [7, 8]) == 0
+    for bad in (t[:50], np.array([5, SMALL.vocab_size])):  # no page; no such token
+        with pytest.raises(_lib.VtbError):
+            st.prefill(bad, 0)
+    for layer in range(SMALL.n_layers):
+        assert st.lib.vtb_cuda_layer_step(st.h, layer) == 0
+    assert st.lib.vtb_cuda_final_step(st.h) == 0
+    logits, arg = np.empty((2, SMALL.vocab_size), np.float32), np.empty(2, np.int32)
+    assert st.lib.vtb_cuda_finalize_token(st.h, logits.ctypes.data, arg.ctypes.data) == 0
+    assert np.array_equal(logits, la) and np.array_equal(arg, aa)
+    assert st.pos(0) == 21 and st.pos(1) == 34
+    ops.check_device_error()

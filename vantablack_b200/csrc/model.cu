@@ -1552,13 +1552,18 @@ int64_t vtb_cuda_state_pos(VtbCudaState* s, int32_t seq) {
 
 // Stage the rows of a step (token, sequence, position) and embed them
 // (gatherEmbedding, forward.zig:163).  Checks mirror stepWithBackend's
-// (forward.zig:159-160) and prefillCpu's (prefill.zig:123-127).
+// (forward.zig:159-160) and prefillCpu's (prefill.zig:123-127).  A call that is
+// refused changes nothing: a token that was begun goes on.
 static int stage_rows(VtbCudaState* s, int rows, const int32_t* tok, const int32_t* seq, const int32_t* pos) {
   const VtbCudaLlamaConfig& c = s->m->c;
   if (rows <= 0 || rows > s->max_rows) return merr(VTB_CUDA_ERR_INVALID_ARG, "too many rows for this state");
   for (int r = 0; r < rows; ++r) {
     if (tok[r] < 0 || tok[r] >= c.vocab_size) return merr(VTB_CUDA_ERR_INVALID_ARG, "token id out of range");
     if (pos[r] >= c.max_seq) return merr(VTB_CUDA_ERR_STREAM_ABORTED, "KV cache full");
+  }
+  if (s->pool)
+    if (const int rc = pool_reserve(s->pool, rows, seq, pos)) return rc;
+  for (int r = 0; r < rows; ++r) {
     s->hbuf[r] = tok[r];
     s->hbuf[s->max_rows + r] = seq[r];
     s->hbuf[2 * s->max_rows + r] = pos[r];
@@ -1570,13 +1575,8 @@ static int stage_rows(VtbCudaState* s, int rows, const int32_t* tok, const int32
   for (int r = 0; r < rows; ++r) s->max_pos = std::max(s->max_pos, (int)pos[r]);
   s->one_seq = true;
   for (int r = 1; r < rows; ++r) s->one_seq = s->one_seq && seq[r] == seq[0];
-  if (PagePool* p = s->pool) {
+  if (s->pool) {
     // rows are one token of each sequence in order (decode), or consecutive tokens of one (prefill)
-    int rc = pool_reserve(p, rows, seq, pos);
-    if (rc) {
-      s->rows = 0;
-      return rc;
-    }
     int32_t *lens = s->hbuf + 3 * (size_t)s->max_rows, *starts = lens + s->n_seqs;
     for (int q = 0, r = 0; q < s->n_seqs; ++q) {
       lens[q] = (int32_t)s->seq_pos[q];
