@@ -389,7 +389,10 @@ void vtb_cuda_state_destroy(VtbCudaState *s);
  * positions and its first `sinks`, and pages left behind by the window are given
  * back.  head_dim 64 or 128, one GPU.  Every call on states works on it; a step
  * or prefill that finds no free page fails with -7 before it changes anything
- * (vtb_cuda_prefill in chunks of max_rows: before the chunk that finds none). */
+ * (vtb_cuda_prefill in chunks of max_rows: before the chunk that finds none).
+ * Token -1 in vtb_cuda_step or vtb_cuda_begin_token leaves that sequence idle (one
+ * that was released or is at its end, say): it takes no page, keeps its position,
+ * its argmax is -1 and its row of logits means nothing. */
 typedef struct VtbCudaPagedConfig {
   int32_t page_size, n_pages, kv_type, window, sinks;
 } VtbCudaPagedConfig;

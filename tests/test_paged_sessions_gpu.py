@@ -1,5 +1,5 @@
-"""Sessions on a paged state: a windowed prompt behind queued work, prompts in chunks under a window, head_dim 128,
-and calls that are refused in the middle of a token."""
+"""Sessions on a paged state: a windowed prompt behind queued work, prompts in chunks under a window, sequences that
+stay idle, and calls that are refused in the middle of a token."""
 import numpy as np
 import pytest
 
@@ -89,6 +89,81 @@ def test_head_dim_128_against_the_oracle():
         assert near(b[0], a, LOGITS) and y[0] == O.argmax(a)
     ops.check_device_error()
     m.close()
+
+
+@pytest.mark.parametrize("graph", [True, False])
+@pytest.mark.parametrize("kv_type", [S.F32, S.BF16])
+def test_idle_sequences(model, kv_type, graph):
+    """Token -1 leaves a sequence out of a step: it takes no page, keeps its position, and the others are as alone."""
+    tol = LOGITS if kv_type == S.F32 else 16 * 2.0 ** -8
+    st = CudaState(model, 3, 64, paged=PagedConfig(20, 8, kv_type))
+    alone = [CudaState(model, 1, 64, paged=PagedConfig(20, 8, kv_type)) for _ in range(3)]
+    t = tokens(200, 12)
+    for s, n in ((0, 20), (1, 31), (2, 5)):
+        st.prefill(t[:n], s)
+        alone[s].prefill(t[:n])
+    at = 40
+
+    def step(active):
+        nonlocal at
+        toks = [int(t[at + s]) if s in active else -1 for s in range(3)]
+        at += 3
+        before = [st.pos(s) for s in range(3)]
+        logits, arg = st.step(toks, graph=graph)
+        for s in range(3):
+            if s in active:
+                la, aa = alone[s].step([toks[s]])
+                assert near(logits[s], la[0], tol) and (kv_type != S.F32 or arg[s] == aa[0])
+                assert st.pos(s) == before[s] + 1
+            else:
+                assert st.pos(s) == before[s] and arg[s] == -1
+
+    step({0, 1, 2})
+    st.release(1)
+    held = 20 - st.free_pages() - sum(-(-st.pos(s) // 8) for s in (0, 2))
+    assert held == 0
+    for _ in range(17):
+        step({0, 2})
+        assert 20 - st.free_pages() == sum(-(-st.pos(s) // 8) for s in (0, 2))  # none for sequence 1
+    step({2})
+    step(set())
+    assert st.pos(1) == 0
+    st.prefill(t[100:117], 1)  # a new session in its place
+    alone[1].reset()
+    alone[1].prefill(t[100:117])
+    for _ in range(4):
+        step({0, 1, 2})
+    step({1})
+    ops.check_device_error()
+
+
+def test_idle_sequences_need_nothing(model):
+    """A full pool, and a sequence at its longest, hold up nobody else."""
+    st = CudaState(model, 2, 128, paged=PagedConfig(17, 8))
+    st.prefill(tokens(128, 1), 0)
+    with pytest.raises(_lib.VtbError):
+        st.step([4, 5])  # sequence 0 is full
+    ref = CudaState(model, 1, 128)
+    for tok in tokens(8, 2):
+        (a, x), (b, y) = ref.step([tok]), st.step([-1, tok])
+        assert near(b[1], a[0], LOGITS) and x[0] == y[1]
+    assert st.free_pages() == 0 and st.pos(0) == 128
+    with pytest.raises(_lib.VtbError) as e:
+        st.step([-1, 9])  # no page for sequence 1
+    assert e.value.status == -7 and st.pos(1) == 8
+    st.step([-1, -1])
+    ops.check_device_error()
+
+
+def test_idle_is_for_steps_of_paged_states(model):
+    paged, plain = CudaState(model, 2, 16, paged=PagedConfig(8, 16)), CudaState(model, 2, 16)
+    for st, toks in ((plain, [-1, 4]), (paged, [-2, 4]), (paged, [SMALL.vocab_size, 4])):
+        with pytest.raises(_lib.VtbError):
+            st.step(toks)
+        assert begin(st, toks) == -1
+    with pytest.raises(_lib.VtbError):
+        paged.prefill([3, -1, 4], 0)
+    assert paged.pos(0) == 0 and paged.free_pages() == 8
 
 
 def test_refused_calls_leave_a_begun_token(model):

@@ -1242,6 +1242,7 @@ static void pool_evict(PagePool* p, int s, int64_t pos) {
 static int pool_reserve(PagePool* p, int rows, const int32_t* seq, const int32_t* pos) {
   std::vector<int32_t*> taken;
   for (int r = 0; r < rows; ++r) {
+    if (pos[r] < 0) continue;  // idle
     int32_t& e = p->at(seq[r], pos[r] / p->c.page_size);
     if (e >= 0) continue;
     if (!pool_take(p, seq[r], pos[r])) {
@@ -1553,18 +1554,20 @@ int64_t vtb_cuda_state_pos(VtbCudaState* s, int32_t seq) {
 // Stage the rows of a step (token, sequence, position) and embed them
 // (gatherEmbedding, forward.zig:163).  Checks mirror stepWithBackend's
 // (forward.zig:159-160) and prefillCpu's (prefill.zig:123-127).  A call that is
-// refused changes nothing: a token that was begun goes on.
+// refused changes nothing: a token that was begun goes on.  A negative position
+// (paged states): the sequence is idle, its row goes along as one without keys.
 static int stage_rows(VtbCudaState* s, int rows, const int32_t* tok, const int32_t* seq, const int32_t* pos) {
   const VtbCudaLlamaConfig& c = s->m->c;
   if (rows <= 0 || rows > s->max_rows) return merr(VTB_CUDA_ERR_INVALID_ARG, "too many rows for this state");
   for (int r = 0; r < rows; ++r) {
+    if (pos[r] < 0) continue;
     if (tok[r] < 0 || tok[r] >= c.vocab_size) return merr(VTB_CUDA_ERR_INVALID_ARG, "token id out of range");
     if (pos[r] >= c.max_seq) return merr(VTB_CUDA_ERR_STREAM_ABORTED, "KV cache full");
   }
   if (s->pool)
     if (const int rc = pool_reserve(s->pool, rows, seq, pos)) return rc;
   for (int r = 0; r < rows; ++r) {
-    s->hbuf[r] = tok[r];
+    s->hbuf[r] = pos[r] < 0 ? 0 : tok[r];
     s->hbuf[s->max_rows + r] = seq[r];
     s->hbuf[2 * s->max_rows + r] = pos[r];
   }
@@ -1898,13 +1901,21 @@ extern "C" {
 
 // ---- the backend vtable, one call per slot (backend.zig:67-97) ----
 
+// One token of every sequence; -1 leaves a sequence of a paged state idle.
+static int stage_step(VtbCudaState* s, const int32_t* tokens) {
+  std::vector<int32_t> seq(s->n_seqs), pos(s->n_seqs);
+  for (int i = 0; i < s->n_seqs; ++i) {
+    seq[i] = i;
+    pos[i] = s->pool && tokens[i] == -1 ? -1 : (int32_t)s->seq_pos[i];
+  }
+  return stage_rows(s, s->n_seqs, tokens, seq.data(), pos.data());
+}
+
 int vtb_cuda_begin_token(VtbCudaState* s, const int32_t* tokens) {
   cudaGetLastError();  // drop a stale error left by an unrelated earlier call
   if (!s || !tokens) return merr(VTB_CUDA_ERR_INVALID_ARG, "null argument");
   cudaSetDevice(s->m->device);
-  std::vector<int32_t> seq(s->n_seqs), pos(s->n_seqs);
-  for (int i = 0; i < s->n_seqs; ++i) { seq[i] = i; pos[i] = (int32_t)s->seq_pos[i]; }
-  int rc = stage_rows(s, s->n_seqs, tokens, seq.data(), pos.data());
+  int rc = stage_step(s, tokens);
   if (rc) return rc;
   cudaError_t e = upload_table(s);
   return mcuda(e ? e : enqueue_embed(s));
@@ -1930,6 +1941,10 @@ int vtb_cuda_finalize_token(VtbCudaState* s, float* logits, int32_t* argmax) {
   int rc = finalize(s, n, logits, argmax);
   if (rc == VTB_CUDA_OK)  // cache.advance (forward.zig:168)
     for (int i = 0; i < s->n_seqs; ++i) {
+      if (s->hbuf[2 * s->max_rows + i] < 0) {  // idle
+        if (argmax) argmax[i] = -1;
+        continue;
+      }
       s->seq_pos[i] += 1;
       if (s->pool) pool_evict(s->pool, i, s->seq_pos[i]);
     }
@@ -1944,9 +1959,7 @@ int vtb_cuda_step(VtbCudaState* s, const int32_t* tokens, float* logits, int32_t
   cudaGetLastError();  // drop a stale error left by an unrelated earlier call
   if (!s || !tokens) return merr(VTB_CUDA_ERR_INVALID_ARG, "null argument");
   cudaSetDevice(s->m->device);
-  std::vector<int32_t> seq(s->n_seqs), pos(s->n_seqs);
-  for (int i = 0; i < s->n_seqs; ++i) { seq[i] = i; pos[i] = (int32_t)s->seq_pos[i]; }
-  int rc = stage_rows(s, s->n_seqs, tokens, seq.data(), pos.data());
+  int rc = stage_step(s, tokens);
   if (rc) return rc;
   if (cudaError_t et = upload_table(s)) return mcuda(et);
   if (!s->graph || s->graph_rows != s->rows) {

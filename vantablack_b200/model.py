@@ -378,7 +378,8 @@ class CudaState:
         return bool(self.lib.vtb_cuda_state_tp_p2p(self.h))
 
     def step(self, tokens, want_logits: bool = True, graph: bool = True):
-        """One token per sequence; returns (logits [n_seqs, vocab] or None, argmax [n_seqs])."""
+        """One token per sequence (-1: a sequence of a paged state stays idle); returns (logits [n_seqs, vocab] or
+        None, argmax [n_seqs])."""
         t = np.ascontiguousarray(np.atleast_1d(tokens), np.int32)
         assert t.size == self.n_seqs
         am = np.empty(self.n_seqs, np.int32)
