@@ -274,8 +274,11 @@ def _workspace_bytes(dtype: torch.dtype, n_heads: int, n_kv_heads: int, head_dim
 
 def paged_attention_workspace(dtype: torch.dtype, n_heads: int, n_kv_heads: int, head_dim: int,
                               device="cuda") -> torch.Tensor:
-    """A workspace for the paged attention calls of one stream (calls that may overlap need one each)."""
-    n = _workspace_bytes(dtype, n_heads, n_kv_heads, head_dim, _current_device())
+    """A workspace for the paged attention calls of one stream on `device` (calls that may overlap need one each)."""
+    device = torch.device(device)
+    dev = _current_device() if device.index is None else device.index
+    with torch.cuda.device(dev):  # its size goes by the device's SMs
+        n = _workspace_bytes(dtype, n_heads, n_kv_heads, head_dim, dev)
     return torch.empty(n, dtype=torch.uint8, device=device)
 
 
