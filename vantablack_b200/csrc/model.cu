@@ -933,7 +933,15 @@ struct VtbCudaState {
 // Error text goes to the same thread-local buffer as the rest of the shim
 // (vtb_cuda_last_error); the library is one translation unit.
 static int merr(int st, const char* msg) { return set_err(st, "%s", msg); }
+static thread_local int g_kept = 0;  // status of a failed call of the shim itself, whose text is to stay
+static cudaError_t keep_status(int rc) {
+  g_kept = rc;
+  return rc ? cudaErrorUnknown : cudaSuccess;
+}
 static int mcuda(cudaError_t e) {
+  const int kept = g_kept;
+  g_kept = 0;
+  if (e == cudaErrorUnknown && kept) return kept;
   if (e == cudaErrorUnknown && strncmp(g_last_err, "NCCL", 4) == 0) return VTB_CUDA_ERR_COMM;
   return cuda_status(e);
 }
@@ -1785,7 +1793,7 @@ static cudaError_t enqueue_layer(VtbCudaState* s, int l) {
     int rc = vtb_cuda_paged_append(&kv, &rows, st);
     if (!rc) rc = s->decode_rows && R == s->n_seqs ? vtb_cuda_paged_attn_decode(&kv, &attn, st)
                                                    : vtb_cuda_paged_attn_prefill(&kv, &attn, p->lens + s->n_seqs, R, st);
-    if (rc) return cudaErrorUnknown;
+    if ((e = keep_status(rc))) return e;
     if (p->out) {
       const long long n = (long long)R * qd;
       if (p->c.kv_type == T_F16) widen_kernel<<<dim3((unsigned)((n + 255) / 256)), 256, 0, st>>>((const __half*)p->out, s->att, n);
