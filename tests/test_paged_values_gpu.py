@@ -293,3 +293,29 @@ def test_infinities_at_both_ends_of_a_long_context():
     got[:, 4:8, 5:7] = want[:, 4:8, 5:7]
     assert torch.equal(got, want)
     assert slow <= 10 * clean, f"{slow:.3f} ms, {clean:.3f} without"
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nats", [2.0, 5.0])
+def test_large_values_where_the_maximum_grows(dtype, hd, nats):
+    """V next to the end of the range at a position whose score is above all before it: its weight is 1 at most."""
+    length, n = 700, 40
+    cache = P.Cache([length], 2, hd, 16, dtype, 80)
+    at = 600
+    for head in range(2):
+        for t in range(length):
+            cache.k_rows[0][t, head, 0] = 0.0
+        put(cache, "k", 0, at, head, 0, nats)
+    pg = cache.table[0].cpu().long()[torch.arange(length) // 16].cuda()
+    cache.k[pg, :, torch.arange(length).cuda() % 16, 0] = cache.k_rows[0][:, :, 0].cuda()
+    put(cache, "v", 0, at, 1, 7, 3.0e38)
+    q = torch.zeros(n, 8, hd)
+    q[:, :, 0] = 1.0
+    q[:, :, 1:] = 0.02 * torch.randn(n, 8, hd - 1, generator=torch.Generator().manual_seed(13))
+    q = q.to(dtype).cuda()
+    pos = torch.arange(length - n, length)
+    ref = P.attention(q.double().cpu(), cache.k_rows[0].double(), cache.v_rows[0].double(), pos, 1.0)
+    for r, got in ((ref, prefill(cache, q, 0, n, scale=1.0)), (tuple(x[-1:] for x in ref), decode(cache, q[-1:], scale=1.0))):
+        err = (got.double().cpu() - r[0]).abs()
+        assert bool(torch.isfinite(got.float()).all()) and bool((err <= bound(r, length, dtype)).all())

@@ -191,12 +191,13 @@ template <typename T> __device__ __forceinline__ uint32_t nonfinite2(uint32_t w)
 
 constexpr int TQ = 128, TN = 128, TC_THREADS = 384;
 // How far (in bits) the maximum that P is relative to may lag behind a row's own before O
-// is rescaled, and the power of two that P is kept times.  bf16 has f32's range.  f16
+// is rescaled, and the power of two that P is kept times.  bf16 has f32's range: P is at
+// most 1, so a sum overflows only where the plain one does.  f16
 // ends at steps of 2^-24, so weights far below the largest would be lost from the
 // products, but not from the row's sum: they are kept times 2^13 (2^15 at most, with
 // the lag), which holds them to 2^-38 of the largest.  4096 tokens on 4096 (32 / 8 heads
 // x 128): 522 us; lag 8 and 2^7 (2^-32) 516; no lag and 2^15 (2^-40) 548.
-template <typename T> struct Range { static constexpr float LAG = 8.f, UP = 0.f; };
+template <typename T> struct Range { static constexpr float LAG = 8.f, UP = -8.f; };
 template <> struct Range<__half> { static constexpr float LAG = 2.f, UP = 13.f; };
 // Registers per thread after the split: softmax warps, MMA and gather warps.
 // setmaxnreg draws on what the CTA was launched with, so the sum of the shares
