@@ -187,3 +187,22 @@ def test_refused_calls_leave_a_begun_token(model):
     assert np.array_equal(logits, la) and np.array_equal(arg, aa)
     assert st.pos(0) == 21 and st.pos(1) == 34
     ops.check_device_error()
+
+
+def test_prompt_over_a_token_that_was_given_up(tall):
+    """Layers of a begun token are still queued when a prompt takes its place: they run on the rows and the table that
+    they were queued with, so no page is missing."""
+    n = 512
+    pc = PagedConfig(n + 32, 8)
+    st, want = CudaState(tall, n, n, paged=pc), CudaState(tall, 1, 128, paged=pc)
+    t = np.random.default_rng(6).integers(3, TALL.vocab_size, 100)
+    a, x = want.prefill(t)
+    assert begin(st, [5] * n) == 0
+    for _ in range(200):  # about 30 us each on the device, queued faster than that
+        assert st.lib.vtb_cuda_final_step(st.h) == 0
+    assert begin(st, [6] * n) == 0  # its rows are copied behind them
+    for layer in range(TALL.n_layers):
+        assert st.lib.vtb_cuda_layer_step(st.h, layer) == 0
+    b, y = st.prefill(t)
+    ops.check_device_error()
+    assert near(b, a, LOGITS) and x == y

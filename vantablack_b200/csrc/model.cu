@@ -928,6 +928,7 @@ struct VtbCudaState {
   long long flag_off = 0;   // floats from a block's start to its flags
   int par = 0;              // slot of the next all-reduce (host count mod 2; every call does an even number)
   PagePool* pool = nullptr; // paged cache (vtb_cuda_state_create_paged) in place of kc / vc
+  bool in_flight = false;   // layer steps of a begun token are queued, which read the staged rows
 };
 
 // Error text goes to the same thread-local buffer as the rest of the shim
@@ -1572,6 +1573,11 @@ static int stage_rows(VtbCudaState* s, int rows, const int32_t* tok, const int32
     if (tok[r] < 0 || tok[r] >= c.vocab_size) return merr(VTB_CUDA_ERR_INVALID_ARG, "token id out of range");
     if (pos[r] >= c.max_seq) return merr(VTB_CUDA_ERR_STREAM_ABORTED, "KV cache full");
   }
+  // Layers of a token that was given up read the staged rows and the page table: both
+  // change only behind them.
+  if (s->in_flight)
+    if (const cudaError_t e = cudaStreamSynchronize(s->st)) return mcuda(e);
+  s->in_flight = false;
   if (s->pool)
     if (const int rc = pool_reserve(s->pool, rows, seq, pos)) return rc;
   for (int r = 0; r < rows; ++r) {
@@ -1933,6 +1939,7 @@ int vtb_cuda_layer_step(VtbCudaState* s, int32_t layer) {
   cudaGetLastError();  // drop a stale error left by an unrelated earlier call
   if (!s || layer < 0 || layer >= s->m->c.n_layers || s->rows <= 0)
     return merr(VTB_CUDA_ERR_INVALID_ARG, "bad layer step");
+  s->in_flight = true;
   return mcuda(enqueue_layer(s, layer));
 }
 
@@ -1947,6 +1954,7 @@ int vtb_cuda_finalize_token(VtbCudaState* s, float* logits, int32_t* argmax) {
   if (!s || s->rows <= 0) return merr(VTB_CUDA_ERR_INVALID_ARG, "no token staged");
   const int n = s->rows;
   int rc = finalize(s, n, logits, argmax);
+  if (rc == VTB_CUDA_OK) s->in_flight = false;
   if (rc == VTB_CUDA_OK)  // cache.advance (forward.zig:168)
     for (int i = 0; i < s->n_seqs; ++i) {
       if (s->hbuf[2 * s->max_rows + i] < 0) {  // idle
