@@ -219,8 +219,13 @@ int vtb_cuda_paged_append(const VtbCudaPagedKv *kv, const VtbCudaPagedRows *rows
  * multiple of n_kv_heads, 128 times it at most (query head h reads kv head h / (n_heads / n_kv_heads)).
  * lens[s] counts the cached positions of sequence s, the new ones included.  A
  * query at position p sees t <= p, with window > 0 only t > p - window or
- * t < sinks.  Softmax and sums are in f32.  A query that sees nothing gets zeros; what a
- * query does not see, infinities and NaN included, does not reach its output. */
+ * t < sinks.  Softmax and sums are in f32, and the weights enter the products with f32
+ * caches as two tf32 values, with 16-bit caches as two 16-bit values (2^-17 of a
+ * weight at most), so a 16-bit output carries its own rounding only; of f16 caches
+ * weights below 2^-38 of the largest are lost.  A query that sees nothing gets zeros; what a
+ * query does not see, infinities and NaN included, does not reach its output.  Of
+ * what it sees, a score of -inf weighs nothing, one of inf or NaN makes the output NaN,
+ * and an infinity or NaN in V reaches its value whatever its weight. */
 typedef struct VtbCudaPagedAttn {
   const void *q;
   void *out;
@@ -387,7 +392,8 @@ void vtb_cuda_state_destroy(VtbCudaState *s);
  * they grow (each at most the model's max_seq positions) and given back on
  * release or reset.  window > 0: every query sees its sequence's last `window`
  * positions and its first `sinks`, and pages left behind by the window are given
- * back.  head_dim 64 or 128, one GPU.  Every call on states works on it; a step
+ * back.  head_dim 64 or 128; one GPU (refused under tensor parallelism, with which
+ * it has not been run).  Every call on states works on it; a step
  * or prefill that finds no free page fails with -7 before it changes anything
  * (vtb_cuda_prefill in chunks of max_rows: before the chunk that finds none).
  * Token -1 in vtb_cuda_step or vtb_cuda_begin_token leaves that sequence idle (one

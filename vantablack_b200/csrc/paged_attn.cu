@@ -59,7 +59,7 @@ constexpr float TINY = 1.2e-38f;
 // Measured, with the join: one sequence of 131009 (8 kv heads x 128, bf16, 537 MB)
 // 93 us, the main kernel alone at 6.5 TB/s; 32 sequences of 2049 to 2560 in f32
 // (604 MB) 109 to 121 us, bound by issue (52% active) and the latency of the split
-// products; 61 sequences behind a window of 1024 in f16 (124 MB) 33 us, of which
+// products; 61 sequences behind a window of 1024 in f16 (124 MB) 34 us, of which
 // the plan, the ring's start and the join are half; 37 positions 4.7 us.
 
 template <typename T, int HD, int NT> struct DecodeCfg {

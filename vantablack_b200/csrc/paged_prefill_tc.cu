@@ -31,12 +31,15 @@
 //
 // Bound by the chain of one row tile, not by a pipe: the softmax with its 1024 clocks
 // of exponentials at the MUFU rate and the rounding of both parts of P, then P V (1024
-// clocks at 128 values) and the next Q K^T (512), and the hand-overs.  Measured (32 /
-// 8 heads x 128, bf16): 2048 tokens 64 us (0.53 PFLOP/s), 8192 under a window of 4096
-// 593 us (0.70); 11 chunks of 1 to 511 (32 / 4 x 64, f16) 115 us.  With P as one 16-bit
-// value it was 53, 459 and 96 us, at an error against 64 bits of 0.0020 (bf16) and
-// 2.9e-4 (f16) of the output in place of the 0.0016 and 2.1e-4 that the output's rounding
-// makes alone.
+// clocks at 128 values) and the next Q K^T (512), and the hand-overs.  A pair of row
+// tiles takes 4500 to 4800 clocks per tile of positions at 128 values, 4170 at 64; to
+// that a call adds 18 to 19 us, and the change from one item to the next 10 us (64) to
+// 20 us (128), which no stage of the kernel has been seen to account for.  Measured
+// (32 / 8 heads x 128, bf16): 2048 tokens 64 us (0.53 PFLOP/s), 8192 under a window of
+// 4096 586 to 593 us (0.70); 11 chunks of 1 to 511 (32 / 4 x 64, f16) 112 to 115 us.  With
+// P as one 16-bit value it was 53, 459 and 96 us, at an error against 64 bits of 0.0020
+// (bf16) and 2.9e-4 (f16) of the output in place of the 0.0016 and 2.1e-4 that the
+// output's rounding makes alone.
 //
 // The scale is taken positive (a negative one negates Q in the first product),
 // so the maximum of S is the maximum of the scaled scores.
