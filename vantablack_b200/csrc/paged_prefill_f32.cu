@@ -24,7 +24,7 @@
 // Tensor work of a tile at 128 values: 48 instructions of Q K^T (46 clocks each,
 // measured) and 24 of P V (67), 3.8k clocks; a tile takes 8.5k, as the softmax with
 // its splits follows Q K^T and a second S has no room in TMEM at 128 values.  256
-// tokens on 1797 (32 / 8 heads x 128): 97 to 102 us, 83 TFLOP/s, 250 in tf32 products.
+// tokens on 1797 (32 / 8 heads x 128): 100 to 105 us, 80 TFLOP/s, 240 in tf32 products.
 #include <type_traits>
 
 #include "paged.cuh"
